@@ -16,6 +16,8 @@ from .operations import (
     spherical_harmonics,
     EquivariantTensorProduct,
     Linear,
+    IrrepsNorm,
+    GatedResidual,
 )
 
 from ._lib import check_status  # noqa: E402  (raises if a kernel reported a bounded wait that ran out)

@@ -240,6 +240,29 @@ class GemmF32x3TnArgs(C.Structure):
     ]
 
 
+NORM_MAX_BLOCKS = 64
+NORM_BRANCH, NORM_ALONE, NORM_BOTH = 1, 2, 3
+NORM_GATES = {None: 0, "sigmoid": 1, "silu": 2}
+
+
+class NormBlock(C.Structure):
+    _fields_ = [("mul", C.c_int32), ("dim", C.c_int32)]
+
+
+class NormArgs(C.Structure):
+    _fields_ = [
+        ("struct_bytes", C.c_int32), ("mode", C.c_int32), ("gate", C.c_int32), ("mul_ir", C.c_int32),
+        ("dtype", C.c_int32), ("param_dtype", C.c_int32), ("num_blocks", C.c_int32), ("stats_stride", C.c_int32),
+        ("blocks", C.POINTER(NormBlock)), ("rows", C.c_int64), ("eps", C.c_double),
+        ("x", C.c_void_p), ("y", C.c_void_p), ("g", C.c_void_p), ("h", C.c_void_p), ("go", C.c_void_p), ("gn", C.c_void_p),
+        ("ldx", C.c_int64), ("ldy", C.c_int64), ("ldg", C.c_int64), ("ldh", C.c_int64), ("ldgo", C.c_int64), ("ldgn", C.c_int64),
+        ("scale", C.c_void_p), ("weight", C.c_void_p), ("out", C.c_void_p), ("norm", C.c_void_p),
+        ("dx", C.c_void_p), ("dy", C.c_void_p), ("dg", C.c_void_p), ("dscale", C.c_void_p), ("dweight", C.c_void_p),
+        ("codes", C.c_void_p), ("ld_codes", C.c_int64), ("stats", C.c_void_p), ("parts", C.c_void_p), ("parts_values", C.c_int64),
+        ("status", C.c_void_p),
+    ]
+
+
 _lib = None
 
 
@@ -328,6 +351,11 @@ def lib() -> C.CDLL:
     L.cueq_b200_linear_gw.argtypes = [C.POINTER(LinearArgs), C.c_void_p]
     L.cueq_b200_linear_gw_floats.argtypes = [C.POINTER(LinearArgs)]
     L.cueq_b200_linear_gw_floats.restype = C.c_int64
+    for name in ("code_bytes", "stats", "parts"):
+        getattr(L, f"cueq_b200_norm_{name}").argtypes = [C.POINTER(NormArgs)]
+        getattr(L, f"cueq_b200_norm_{name}").restype = C.c_int64
+    L.cueq_b200_norm_forward.argtypes = [C.POINTER(NormArgs), C.c_void_p]
+    L.cueq_b200_norm_backward.argtypes = [C.POINTER(NormArgs), C.c_void_p]
     L.cueq_b200_selftest_bounded_wait.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
     if L.cueq_b200_abi_version() != 1:
         raise CueqError("libcueq_b200.so has an unexpected ABI version; rebuild it")

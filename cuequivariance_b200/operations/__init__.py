@@ -4,8 +4,10 @@ from .symmetric_contraction import SymmetricContraction
 from .spherical_harmonics import SphericalHarmonics, spherical_harmonics
 from .equivariant import EquivariantTensorProduct
 from .linear import Linear
+from .norm import GatedResidual, IrrepsNorm
 
 __all__ = [
     "ChannelWiseTensorProduct", "FullyConnectedTensorProduct", "SymmetricContraction",
     "SphericalHarmonics", "spherical_harmonics", "EquivariantTensorProduct", "Linear",
+    "IrrepsNorm", "GatedResidual",
 ]

@@ -585,6 +585,56 @@ int cueq_b200_fctp_fused_gw(const cueq_fctp_fused_gw_args* args, void* stream);
  * This is the time-out path of every bounded wait in the tensor-core kernels. */
 int cueq_b200_selftest_bounded_wait(void* status, void* waited_cycles, void* stream);
 
+/* ---- norms around an equivariant block --------------------------------------------------------
+ *
+ * No counterpart in the reference.  Rows of irrep blocks (mul channels x dim components, `mul_ir` or component-major); per row
+ * and block r(t) = (mean of t^2 over the block + eps)^-1/2:
+ *   CUEQ_NORM_BRANCH  out  = x + s act(g) y r(y)      s, g per channel; the gate may be absent
+ *   CUEQ_NORM_ALONE   norm = w x r(x)
+ *   CUEQ_NORM_BOTH    out as above and norm = w out r(out)
+ * Results are dense rows of the features' width (gates: of the number of channels); operands may have rows further apart.
+ * 16- and 32-bit data are computed in 32 bits, 64-bit data in 64; s and w have their own type.
+ *
+ * The forward pass writes `stats` (nullable: nothing is kept), per (row, block) cueq_b200_norm_stats() values of the arithmetic's
+ * type, and with `codes` (16- and 32-bit data) what the backward pass reads of y (alone: x), g and out in 8 bits: rows of ld_codes
+ * bytes, at least cueq_b200_norm_code_bytes().  The backward pass takes the same stats and either codes or the operands
+ * themselves (`h`: x or out), the cotangents go (of out; nullable with BOTH) and gn (of norm), and writes dx (BRANCH: not
+ * written, it is go), dy, dg, dscale, dweight.  `parts`: cueq_b200_norm_parts() values of the arithmetic's type. */
+#define CUEQ_NORM_MAX_BLOCKS 64
+#define CUEQ_NORM_BRANCH 1
+#define CUEQ_NORM_ALONE 2
+#define CUEQ_NORM_BOTH 3
+#define CUEQ_NORM_GATE_NONE 0
+#define CUEQ_NORM_GATE_SIGMOID 1
+#define CUEQ_NORM_GATE_SILU 2
+typedef struct { int32_t mul, dim; } cueq_norm_block;
+typedef struct {
+  int32_t struct_bytes;          /* sizeof(cueq_norm_args)                                          */
+  int32_t mode, gate, mul_ir;    /* CUEQ_NORM_*; mul_ir: 1, component-major: 0                      */
+  int32_t dtype, param_dtype;    /* CUEQ_F32 ..: features and gates; s, w and their gradients       */
+  int32_t num_blocks;
+  int32_t stats_stride;          /* statistics per (row, block); 0: what this mode writes             */
+  const cueq_norm_block* blocks; /* HOST array                                                      */
+  int64_t rows;
+  double eps;
+  const void *x, *y, *g, *h, *go, *gn;
+  int64_t ldx, ldy, ldg, ldh, ldgo, ldgn;   /* elements from row to row                             */
+  const void *scale, *weight;
+  void *out, *norm;
+  void *dx, *dy, *dg, *dscale, *dweight;
+  void* codes;
+  int64_t ld_codes;              /* bytes, a multiple of 16                                         */
+  void* stats;
+  void* parts;
+  int64_t parts_values;
+  void* status;                  /* nullable device int32: 2 if a bounded wait ran out              */
+} cueq_norm_args;
+int64_t cueq_b200_norm_code_bytes(const cueq_norm_args* args);
+int64_t cueq_b200_norm_stats(const cueq_norm_args* args);
+int64_t cueq_b200_norm_parts(const cueq_norm_args* args);
+int cueq_b200_norm_forward(const cueq_norm_args* args, void* stream);
+int cueq_b200_norm_backward(const cueq_norm_args* args, void* stream);
+
 /* ---- channelwise forward for callers that cannot allocate ----------------------------------
  *
  * No counterpart in the reference.  cueq_b200_cw_forward expects the caller to keep the CSR row
