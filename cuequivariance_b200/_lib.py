@@ -232,6 +232,13 @@ class LinearArgs(C.Structure):
     ]
 
 
+class LinearCodes(C.Structure):
+    _fields_ = [
+        ("struct_bytes", C.c_int32), ("reserved", C.c_int32), ("rows", C.c_int64), ("codes", C.c_void_p), ("ld_codes", C.c_int64),
+        ("steps", C.c_void_p), ("ld_steps", C.c_int64),
+    ]
+
+
 class GemmF32x3TnArgs(C.Structure):
     _fields_ = [
         ("A", C.c_void_p), ("B", C.c_void_p), ("C", C.c_void_p), ("colsum", C.c_void_p),
@@ -349,6 +356,8 @@ def lib() -> C.CDLL:
     L.cueq_b200_fctp_gw_floats.restype = C.c_int64
     L.cueq_b200_linear_map.argtypes = [C.POINTER(LinearArgs), C.c_void_p]
     L.cueq_b200_linear_gw.argtypes = [C.POINTER(LinearArgs), C.c_void_p]
+    L.cueq_b200_linear_pack.argtypes = [C.POINTER(LinearArgs), C.POINTER(LinearCodes), C.c_void_p]
+    L.cueq_b200_linear_gw_codes.argtypes = [C.POINTER(LinearArgs), C.POINTER(LinearCodes), C.c_void_p]
     L.cueq_b200_linear_gw_floats.argtypes = [C.POINTER(LinearArgs)]
     L.cueq_b200_linear_gw_floats.restype = C.c_int64
     for name in ("code_bytes", "stats", "parts"):

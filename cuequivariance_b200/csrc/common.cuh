@@ -61,6 +61,18 @@ __device__ __forceinline__ int64_t load_index(const void* idx, int is64, int64_t
               : (int64_t)__ldg(reinterpret_cast<const int*>(idx) + z);
 }
 
+// Activations kept in 8 bits: code = rint(v / step), step the smallest power of two (at least 2^-126) of which 127 hold the block's
+// largest magnitude.  A power of two costs at most one of the seven bits, code * step is exact in bf16 and TF32, and no code depends on
+// how a quotient is rounded.  `top`: bits of the largest magnitude, 127 = 1.984375 * 2^6; an infinity or NaN: step NaN, codes 0.
+__device__ __forceinline__ void code_step(unsigned top, float& step, float& inverse) {
+  if (top >= 0x7f800000u) { step = __uint_as_float(0x7fc00000u); inverse = 0.f; return; }
+  int k = (int)(top >> 23) - 6 + ((top & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+  k = k < 1 ? 1 : k;
+  step = __uint_as_float((unsigned)k << 23);
+  inverse = __uint_as_float((unsigned)(254 - k) << 23);
+}
+__device__ __forceinline__ signed char to_code(float v, float inverse) { return (signed char)__float2int_rn(v * inverse); }
+
 template <typename M>
 __device__ __forceinline__ M warp_sum(M v) {
 #pragma unroll

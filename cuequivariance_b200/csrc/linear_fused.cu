@@ -5,6 +5,10 @@
 //   linear_map  out[z, v, i] = c * sum_u W[class(z)][u, v] x[z, u, i]       forward, and with W transposed the input gradient
 //   linear_gw   gW[class][u, v] += c * sum_{z in class, i} x[z, u, i] g[z, v, i]      partial sums, added in a fixed order
 //
+// x may be kept in 8 bits for the weight gradient: per row and irrep, x ~ step * code (linear_pack).  The codes are exact in TF32, so
+// the sum over them takes two passes (code * g_hi, code * g_lo) and no rounding on that side; the step, a power of two, goes
+// into g.
+//
 // What bounds them: the rows are read once and written once, 2 * 268 MB each for 32,768 nodes of 128x(0e+1o+2e+3o);
 // 82 us at 6.5 TB/s against 46 us of three-pass TF32.  The layer used to be one GEMM launch per irrep and component
 // (48 of them, the row reductions on 32 thread blocks), with layout transpositions around them and the weights split by
@@ -37,7 +41,7 @@ constexpr int kMaxPaths = CUEQ_LINEAR_MAX_PATHS, kMaxClasses = CUEQ_LINEAR_MAX_C
 constexpr int kBlk = 128 * 128;              // one operand block: 128 rows x 32 float32, 16 KiB
 constexpr int kMaxRunGw = 128;               // K blocks per run of linear_gw
 
-struct LPath { int x_off, o_off, w_off, K, N, d, w_sn, w_sk; float c; };
+struct LPath { int x_off, o_off, w_off, K, N, d, w_sn, w_sk; float c; int code_off; };
 
 struct LParams {
   const float* x;       // linear_map: input rows; linear_gw: x rows (M side)
@@ -46,6 +50,9 @@ struct LParams {
   float* parts;         // linear_gw: partial sums, one slot of `slot` floats per run
   int64_t slot;
   const float* g;       // linear_gw: cotangent rows (N side)
+  const signed char* codes;   // linear_gw: x in 8 bits, rows of ldc bytes
+  const float* steps;   // [path][ld_steps], one per row
+  int64_t ldc, ld_steps;
   int64_t ldx, ldo, w_class_stride;
   int x_mul_ir, o_mul_ir, num_paths, num_classes;
   int total;            // tiles (linear_map) or K blocks (linear_gw) over all paths and classes
@@ -437,6 +444,43 @@ __device__ __forceinline__ void gw_transpose(const float* raw, unsigned char* hi
   }
 }
 
+// x in 8 bits -> K-major tile: a code is exact, so there is no lo half
+template <int D, bool MUL_IR>
+__device__ __forceinline__ void gw_transpose_codes(const signed char* raw, unsigned char* hi, int C, int nodes, int tid) {
+  const int ch = tid & 127;
+  if (ch >= C) return;
+#pragma unroll
+  for (int gg = 0; gg < 2; ++gg) {
+    const int chunk = (tid >> 7) * 2 + gg;
+    float v[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int k = chunk * 4 + c, z = k / D, i = k - z * D;
+      v[c] = (z < rows_per_block(D) && z < nodes) ? (float)raw[z * (C * D) + (MUL_IR ? ch * D + i : i * C + ch)] : 0.f;
+    }
+    *reinterpret_cast<float4*>(hi + ch * 128 + ((chunk ^ (ch & 7)) << 4)) = make_float4(v[0], v[1], v[2], v[3]);
+  }
+}
+// g rows times the steps of their nodes -> K-major split tile
+template <int D, bool MUL_IR>
+__device__ __forceinline__ void gw_transpose_steps(const float* raw, unsigned char* hi, int C, int nodes, int tid, const float* steps) {
+  const int ch = tid & 127;
+  if (ch >= C) return;
+#pragma unroll
+  for (int gg = 0; gg < 2; ++gg) {
+    const int chunk = (tid >> 7) * 2 + gg;
+    float v[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int k = chunk * 4 + c, z = k / D, i = k - z * D;
+      v[c] = (z < rows_per_block(D) && z < nodes) ? raw[z * (C * D) + (MUL_IR ? ch * D + i : i * C + ch)] * steps[z] : 0.f;
+    }
+    store_split(hi, hi + kBlk, ch, chunk, v);
+  }
+}
+constexpr int kGwSteps = kBlk - 256;     // the steps of a block's nodes, behind the codes: 4 KiB of codes at most, 40 steps at most
+
+template <bool CODES>
 __global__ void __launch_bounds__(kGwThreads, 1) linear_gw_kernel(const __grid_constant__ LParams p) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -502,8 +546,8 @@ __global__ void __launch_bounds__(kGwThreads, 1) linear_gw_kernel(const __grid_c
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
           const unsigned char* st = base + kGwOps + s * 4 * kBlk;
-          umma_block(tmem_base + 3 * 128, st + kBlk, st + 2 * kBlk, idesc, b ? 1u : 0u);
-          umma_block(tmem_base + 3 * 128, st, st + 3 * kBlk, idesc, 1u);
+          if (!CODES) umma_block(tmem_base + 3 * 128, st + kBlk, st + 2 * kBlk, idesc, b ? 1u : 0u);
+          umma_block(tmem_base + 3 * 128, st, st + 3 * kBlk, idesc, !CODES || b ? 1u : 0u);
           umma_block(tmem_base + (b % 3) * 128, st, st + 2 * kBlk, idesc, b >= 3 ? 1u : 0u);
           umma_commit(opempty + s);
         }
@@ -516,9 +560,12 @@ __global__ void __launch_bounds__(kGwThreads, 1) linear_gw_kernel(const __grid_c
     bool ok = true;
     for_each_run(p, first, last, rows_per_block, [&](const LPath& q, int, int z0, int zend, int blocks) {
       const int n = rows_per_block(q.d);
-      const unsigned bytes = (unsigned)((is_g ? q.N : q.K) * q.d * 4);
-      const int64_t ld = is_g ? p.ldo : p.ldx;
-      const float* src = (is_g ? p.g + q.o_off : p.x + q.x_off) + (int64_t)z0 * ld;
+      const bool codes = CODES && !is_g;
+      const unsigned bytes = (unsigned)((is_g ? q.N : q.K) * q.d * (codes ? 1 : 4));
+      const int64_t ld = codes ? p.ldc : 4 * (is_g ? p.ldo : p.ldx);                   // bytes
+      const unsigned char* src = (codes ? (const unsigned char*)p.codes + q.code_off
+                                        : (const unsigned char*)(is_g ? p.g + q.o_off : p.x + q.x_off)) + (int64_t)z0 * ld;
+      const float* steps = codes ? p.steps + (&q - p.path) * p.ld_steps : nullptr;
       for (int b = 0; b < blocks && ok; ++b, ++it, src += n * ld) {
         const unsigned s = it % kGwRawStages;
         ok = bar_wait(rawempty + s, ((it / kGwRawStages) & 1) ^ 1, p.status);
@@ -526,8 +573,13 @@ __global__ void __launch_bounds__(kGwThreads, 1) linear_gw_kernel(const __grid_c
         if (!ok) break;
         const int nodes = min(n, zend - (z0 + b * n));
         const unsigned raw = s32(base + kGwRaw + s * 2 * kBlk + (is_g ? kBlk : 0));
-        if (lane == 0) bar_expect_tx(rawfull + s, nodes * bytes);
+        // steps: whole groups of four, the first and the last may hold other nodes' as well
+        const int s0 = (z0 + b * n) & ~3, s1 = (z0 + b * n + nodes + 3) & ~3;
+        if (lane == 0) bar_expect_tx(rawfull + s, nodes * bytes + (codes ? (s1 - s0) * 4 : 0));
         __syncwarp();
+        if (codes && lane == 0)
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+                       ::"r"(raw + kGwSteps), "l"(steps + s0), "r"((s1 - s0) * 4), "r"(s32(rawfull + s)) : "memory");
         if (lane < nodes)                                            // one node per lane; at most 32 / d of them
           asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
                        ::"r"(raw + lane * bytes), "l"(src + lane * ld), "r"(bytes), "r"(s32(rawfull + s)) : "memory");
@@ -547,8 +599,14 @@ __global__ void __launch_bounds__(kGwThreads, 1) linear_gw_kernel(const __grid_c
         unsigned char* st = base + kGwOps + s * 4 * kBlk;
         const int nodes = min(n, zend - (z0 + b * n));
         if (!dead) {
-          LINEAR_DISPATCH(gw_transpose, q.d, p.x_mul_ir, raw, st, q.K, nodes, tid)
-          LINEAR_DISPATCH(gw_transpose, q.d, p.o_mul_ir, raw + kBlk / 4, st + 2 * kBlk, q.N, nodes, tid)
+          if (CODES) {
+            const float* steps = raw + kGwSteps / 4 + ((z0 + b * n) & 3);
+            LINEAR_DISPATCH(gw_transpose_codes, q.d, p.x_mul_ir, reinterpret_cast<const signed char*>(raw), st, q.K, nodes, tid)
+            LINEAR_DISPATCH(gw_transpose_steps, q.d, p.o_mul_ir, raw + kBlk / 4, st + 2 * kBlk, q.N, nodes, tid, steps)
+          } else {
+            LINEAR_DISPATCH(gw_transpose, q.d, p.x_mul_ir, raw, st, q.K, nodes, tid)
+            LINEAR_DISPATCH(gw_transpose, q.d, p.o_mul_ir, raw + kBlk / 4, st + 2 * kBlk, q.N, nodes, tid)
+          }
         }
         publish(opfull + s, lane);
         if (lane == 0) bar_arrive(rawempty + r);
@@ -659,9 +717,98 @@ extern "C" int cueq_b200_linear_map(const cueq_linear_args* a, void* stream) {
   return 0;
 }
 
-extern "C" int cueq_b200_linear_gw(const cueq_linear_args* a, void* stream) {
+namespace {
+
+// x rows -> codes and steps, a warp per row and irrep: per block of u * d values the smallest power of two of which 127 hold the
+// largest magnitude (as in norm_kernels.cuh; NaN for a block that holds an infinity or NaN).  268 MB in, 67 MB out for 32,768 nodes
+// of 128x(0e+1o+2e+3o).
+struct PackParams {
+  const float* x;
+  signed char* codes;
+  float* steps;
+  int64_t ldx, ldc, ld_steps, rows;
+  int num_paths;
+  struct { int off, n, code_off; } path[kMaxPaths];
+};
+constexpr int kPackWarps = 8;
+__global__ void __launch_bounds__(32 * kPackWarps) linear_pack_kernel(const __grid_constant__ PackParams p) {
+  const int k = blockIdx.x % p.num_paths, lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)(blockIdx.x / p.num_paths) * kPackWarps + (threadIdx.x >> 5);
+  if (row >= p.rows) return;
+  const int n4 = p.path[k].n / 4;                                    // 224 at most
+  const float4* src = reinterpret_cast<const float4*>(p.x + row * p.ldx + p.path[k].off);
+  float4 v[7];
+  unsigned top = 0;
+#pragma unroll
+  for (int j = 0; j < 7; ++j) v[j] = lane + 32 * j < n4 ? __ldg(src + lane + 32 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+  auto bits = [](float f) { return __float_as_uint(f) & 0x7fffffffu; };
+#pragma unroll
+  for (int j = 0; j < 7; ++j) top = max(top, max(max(bits(v[j].x), bits(v[j].y)), max(bits(v[j].z), bits(v[j].w))));
+  float step, inv;
+  cueq::code_step(__reduce_max_sync(0xffffffffu, top), step, inv);
+  char4* dst = reinterpret_cast<char4*>(p.codes + row * p.ldc + p.path[k].code_off);
+#pragma unroll
+  for (int j = 0; j < 7; ++j)
+    if (lane + 32 * j < n4)
+      dst[lane + 32 * j] = make_char4(cueq::to_code(v[j].x, inv), cueq::to_code(v[j].y, inv), cueq::to_code(v[j].z, inv), cueq::to_code(v[j].w, inv));
+  if (lane == 0) p.steps[k * p.ld_steps + row] = step;
+}
+
+// blocks of codes in the order of the paths, one behind the other; multiples of 32 bytes each
+int code_offsets(const cueq_linear_args* a, int (&off)[kMaxPaths]) {
+  int at = 0;
+  for (int k = 0; k < a->num_paths; ++k) { off[k] = at; at += a->paths[k].u * a->paths[k].d; }
+  return at;
+}
+int check_codes(const cueq_linear_args* a, const cueq_linear_codes* c, int (&off)[kMaxPaths]) {
+  if (!c || c->struct_bytes != (int)sizeof(cueq_linear_codes)) return cueq::fail("linear: codes are missing or the binding declares another block");
+  const int bytes = code_offsets(a, off);
+  if (c->rows < 0 || (c->rows && (!c->codes || !c->steps))) return cueq::fail("linear: null codes or steps");
+  if (c->ld_codes < bytes || c->ld_codes % 16 || c->ld_steps < c->rows || c->ld_steps % 4 || (((uintptr_t)c->codes | (uintptr_t)c->steps) & 15))
+    return cueq::fail("linear: rows of codes need %d bytes, each path a step per row, 16-byte aligned", bytes);
+  if (a->bounds[a->num_classes] > c->rows) return cueq::fail("linear: class bounds beyond the rows of the codes");
+  return 0;
+}
+
+int launch_gw(const cueq_linear_args* a, const cueq_linear_codes* codes, void* stream);
+
+}  // namespace
+
+extern "C" int cueq_b200_linear_gw(const cueq_linear_args* a, void* stream) { return launch_gw(a, nullptr, stream); }
+extern "C" int cueq_b200_linear_gw_codes(const cueq_linear_args* a, const cueq_linear_codes* c, void* stream) {
+  if (!c) return cueq::fail("linear: codes are missing or the binding declares another block");
+  return launch_gw(a, c, stream);
+}
+
+extern "C" int cueq_b200_linear_pack(const cueq_linear_args* a, const cueq_linear_codes* c, void* stream) {
+  LParams p;
+  int off[kMaxPaths];
+  if (int rc = make_params(a, rows_per_block, true, &p)) return rc;
+  if (int rc = check_codes(a, c, off)) return rc;
+  if (c->rows == 0) return 0;
+  const int64_t groups = (c->rows + kPackWarps - 1) / kPackWarps;
+  if (groups * a->num_paths > 2147483647LL) return cueq::fail("linear: too many rows");
+  PackParams q;
+  q.x = p.x; q.codes = (signed char*)c->codes; q.steps = (float*)c->steps;
+  q.ldx = p.ldx; q.ldc = c->ld_codes; q.ld_steps = c->ld_steps; q.rows = c->rows; q.num_paths = a->num_paths;
+  for (int k = 0; k < a->num_paths; ++k) { q.path[k].off = a->paths[k].x_off; q.path[k].n = a->paths[k].u * a->paths[k].d; q.path[k].code_off = off[k]; }
+  linear_pack_kernel<<<(unsigned)(groups * a->num_paths), 32 * kPackWarps, 0, reinterpret_cast<cudaStream_t>(stream)>>>(q);
+  CUEQ_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+
+namespace {
+
+int launch_gw(const cueq_linear_args* a, const cueq_linear_codes* codes, void* stream) {
   LParams p;
   if (int rc = make_params(a, rows_per_block, true, &p)) return rc;
+  if (codes) {
+    int off[kMaxPaths];
+    if (int rc = check_codes(a, codes, off)) return rc;
+    p.codes = (const signed char*)codes->codes; p.steps = (const float*)codes->steps;
+    p.ldc = codes->ld_codes; p.ld_steps = codes->ld_steps;
+    for (int k = 0; k < a->num_paths; ++k) p.path[k].code_off = off[k];
+  }
   p.g = (const float*)a->w;
   p.out = (float*)a->out;
   if (p.total == 0) return 0;
@@ -682,14 +829,17 @@ extern "C" int cueq_b200_linear_gw(const cueq_linear_args* a, void* stream) {
       t.start[s + 1] = at;
     }
   }
-  static cueq::PerDeviceFlag configured;
-  if (!configured.get()) {
-    CUEQ_CUDA_OK(cudaFuncSetAttribute(linear_gw_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGwSmem));
-    configured.set();
+  static cueq::PerDeviceFlag configured[2];
+  const auto kernel = codes ? linear_gw_kernel<true> : linear_gw_kernel<false>;
+  if (!configured[codes != nullptr].get()) {
+    CUEQ_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGwSmem));
+    configured[codes != nullptr].set();
   }
-  linear_gw_kernel<<<grid, kGwThreads, kGwSmem, reinterpret_cast<cudaStream_t>(stream)>>>(p);
+  kernel<<<grid, kGwThreads, kGwSmem, reinterpret_cast<cudaStream_t>(stream)>>>(p);
   CUEQ_CUDA_OK(cudaGetLastError());
   linear_gw_sum_kernel<<<dim3((widest / 4 + 127) / 128, p.num_paths * p.num_classes), 128, 0, reinterpret_cast<cudaStream_t>(stream)>>>(p, t, grid);
   CUEQ_CUDA_OK(cudaGetLastError());
   return 0;
 }
+
+}  // namespace

@@ -19,9 +19,8 @@
 //
 // Sums, statistics and all arithmetic are in 32 bits for 16- and 32-bit data, in 64 for 64-bit data; results are rounded once.
 //
-// Kept in 8 bits (Q8): code = rint(t 2^-k) per (row, irrep block), the smallest k with 127 * 2^k >= max |t|.  A power of two costs
-// at most one of the seven bits, and the codes do not depend on how a quotient is rounded.  A block that holds an infinity or NaN has
-// step NaN, so that its gradients are NaN as well.  r stays that of the exact values.
+// Kept in 8 bits (Q8): codes per (row, irrep block), see code_step in common.cuh.  r stays that of the exact values; the gradients of a block
+// that holds an infinity or NaN are NaN.
 #pragma once
 #include "common.cuh"
 #include "tc_common.cuh"
@@ -134,15 +133,8 @@ __device__ __forceinline__ void activation(int gate, M g, M& v, M& dv) {
   else { v = g * e; dv = e * (M(1) + g * (M(1) - e)); }
 }
 
-// step 2^k and its inverse from the bits of the largest magnitude: 127 = 1.984375 * 2^6
-__device__ __forceinline__ void code_step(unsigned top, float& step, float& inverse) {
-  if (top >= 0x7f800000u) { step = __uint_as_float(0x7fc00000u); inverse = 0.f; return; }
-  int k = (int)(top >> 23) - 6 + ((top & 0x7fffffu) > 0x7e0000u ? 1 : 0);
-  k = k < 1 ? 1 : k;
-  step = __uint_as_float((unsigned)k << 23);
-  inverse = __uint_as_float((unsigned)(254 - k) << 23);
-}
-__device__ __forceinline__ signed char to_code(float v, float inverse) { return (signed char)__float2int_rn(v * inverse); }
+using cueq::code_step;
+using cueq::to_code;
 __device__ __forceinline__ signed char to_code(double, float) { return 0; }
 
 // ---- a thread block's view of its work --------------------------------------------------------------------------------

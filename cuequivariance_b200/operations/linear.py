@@ -12,6 +12,7 @@ from .. import _lib, descriptors
 from ..irreps import Irreps, IrrepsLayout
 from ..segmented_polynomial import SegmentedPolynomial
 from ..transpose import TransposeIrrepsLayout
+from .norm import check_saved_activations
 
 
 DENSE_ROUTE = True      # float32, one weight set, multiplicities that are multiples of 32: tensor-core GEMMs
@@ -176,8 +177,13 @@ class _FusedLinear(torch.autograd.Function):
     in the caller's layouts.  ``bounds``: row ranges of the classes, ``(0, rows)`` for one weight set."""
 
     @staticmethod
-    def _launch(plan, which, bounds, x, w, out, transposed=0):
+    def _launch(plan, which, bounds, x, w, out, transposed=0, codes=None):
+        """``which``: map, gw (``w``: cotangent rows), pack (``w``, ``out``: anything).  ``codes``: written by pack; gw reads them in place
+        of ``x``."""
         import ctypes as C
+
+        if x.shape[0] == 0:
+            return
 
         from .. import profiling
 
@@ -188,28 +194,42 @@ class _FusedLinear(torch.autograd.Function):
         a.num_paths, a.num_classes = len(plan["paths"]), len(bounds) - 1
         a.x_mul_ir, a.out_mul_ir = plan["mul_ir"] if not transposed else plan["mul_ir"][::-1]
         a.transposed, a.struct_bytes = transposed, C.sizeof(a)
-        a.ldx, a.ldo = x.shape[1], (out if which == "map" else w).shape[1]
+        a.ldx, a.ldo = plan["in_size"] if codes is not None else x.shape[1], (out if which == "map" else w).shape[1]
         a.w_class_stride = (w if which == "map" else out).shape[1]
         for q, (wo, u, v, xo, oo, d, c) in zip(a.paths, plan["paths"]):
             q.u, q.v, q.d, q.x_off, q.out_off, q.w_off, q.c = u, v, d, xo, oo, wo, c
         L = _lib.lib()
-        fn = L.cueq_b200_linear_map if which == "map" else L.cueq_b200_linear_gw
+        stream = C.c_void_p(torch.cuda.current_stream(x.device).cuda_stream)
+        if codes is not None:
+            values, steps = codes
+            c = _lib.LinearCodes()
+            c.struct_bytes, c.rows = C.sizeof(c), values.shape[0]
+            c.codes, c.ld_codes, c.steps, c.ld_steps = values.data_ptr(), values.shape[1], steps.data_ptr(), steps.shape[1]
+            gw_codes = L.cueq_b200_linear_pack if which == "pack" else L.cueq_b200_linear_gw_codes
+            fn = lambda args, stream: gw_codes(args, C.byref(c), stream)  # noqa: E731
+        else:
+            fn = L.cueq_b200_linear_map if which == "map" else L.cueq_b200_linear_gw
         parts = None
         if which == "gw":
             n = L.cueq_b200_linear_gw_floats(C.byref(a))
             parts = torch.empty(max(n, 0), dtype=torch.float32, device=x.device)
             a.parts, a.parts_floats = parts.data_ptr(), n
-        name = ("linear" if len(bounds) == 2 else "indexed_linear") + "_f32x3" + ("_gx" if transposed else "" if which == "map" else "_gw")
+        name = ("linear" if len(bounds) == 2 else "indexed_linear") + "_f32x3" + ("_gx" if transposed else "" if which == "map" else f"_{which}")
         with torch.cuda.device(x.device), profiling.kernel(name):
-            _lib.check(fn(C.byref(a), C.c_void_p(torch.cuda.current_stream(x.device).cuda_stream)))
+            _lib.check(fn(C.byref(a), stream))
 
     @staticmethod
-    def forward(ctx, plan, bounds, weight, x):
+    def _apply(plan, bounds, weight, x):
         x, weight = _aligned(x), _aligned(weight)
         all_rows = bounds[0] == 0 and bounds[-1] == x.shape[0]
         out = (torch.empty if plan["full_out"] and all_rows else torch.zeros)((x.shape[0], plan["out_size"]), dtype=torch.float32, device=x.device)
         _FusedLinear._launch(plan, "map", bounds, x, weight, out)
-        ctx.plan, ctx.bounds, ctx.all_rows = plan, bounds, all_rows
+        return out, weight, x, all_rows
+
+    @staticmethod
+    def forward(ctx, plan, bounds, weight, x):
+        out, weight, x, ctx.all_rows = _FusedLinear._apply(plan, bounds, weight, x)
+        ctx.plan, ctx.bounds = plan, bounds
         ctx.save_for_backward(weight, x)
         return out
 
@@ -230,6 +250,38 @@ class _FusedLinear(torch.autograd.Function):
         return None, None, gw, gx
 
 
+class _FusedLinear8(torch.autograd.Function):
+    """``_FusedLinear`` that keeps x in 8 bits: a quarter of the bytes, and a weight gradient of two tensor-core passes, not three."""
+
+    @staticmethod
+    def forward(ctx, plan, bounds, weight, x):
+        out, weight, x, ctx.all_rows = _FusedLinear._apply(plan, bounds, weight, x)
+        ctx.plan, ctx.bounds, ctx.rows = plan, bounds, x.shape[0]
+        values = steps = None
+        if ctx.needs_input_grad[2]:
+            rows, paths = x.shape[0], plan["paths"]
+            values = torch.empty((rows, sum(u * d for (_, u, _, _, _, d, _) in paths)), dtype=torch.int8, device=x.device)
+            steps = torch.empty((len(paths), (rows + 3) // 4 * 4), dtype=torch.float32, device=x.device)
+            _FusedLinear._launch(plan, "pack", bounds, x, x, x, codes=(values, steps))
+        ctx.save_for_backward(weight, values, steps)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gout):
+        plan, bounds = ctx.plan, ctx.bounds
+        weight, values, steps = ctx.saved_tensors
+        gout = _aligned(gout)
+        gw = gx = None
+        if ctx.needs_input_grad[3]:
+            gx = (torch.empty if plan["full_in"] and ctx.all_rows else torch.zeros)((ctx.rows, plan["in_size"]), dtype=torch.float32, device=gout.device)
+            _FusedLinear._launch(plan, "map", bounds, gout, weight, gx, transposed=1)
+        if ctx.needs_input_grad[2]:
+            gw = (torch.empty_like if bounds[-1] > bounds[0] else torch.zeros_like)(weight)
+            _FusedLinear._launch(plan, "gw", bounds, values, gout, gw, codes=(values, steps))
+        return None, None, gw, gx
+
+
 class Linear(torch.nn.Module):
     """``forward(x, weight=None, weight_indices=None)``; ``x``: ``[batch, irreps_in.dim]``;
     ``weight``: ``[1 or weight_classes, weight_numel]`` when shared (the module's own parameter
@@ -240,7 +292,12 @@ class Linear(torch.nn.Module):
     tensor-core launch per result, all irreps and (sorted) weight classes included (``csrc/linear_fused.cu``); other
     multiples of 32 as one GEMM per irrep and component (``dense.gemm_f32x3`` / ``gemm_f32x3_tn``); first derivatives
     only.  Everything else runs on the generic kernel over the polynomial ``uv,iu,iv``
-    flattened over ``u``.  There is no ``naive`` method and no fallback."""
+    flattened over ``u``.  There is no ``naive`` method and no fallback.
+
+    ``saved_activations="int8"`` keeps x in 8 bits for the weight gradient, per row and irrep block with a step of a power of two (off
+    by at most 1/127 of the block's largest magnitude); the output and the input gradient do not change, the weight gradient is that of the kept
+    values.  It is for what the fused launches take (first sentence above, any number of rows); other shapes, types and unsorted
+    classes raise."""
 
     def __init__(
         self,
@@ -258,6 +315,7 @@ class Linear(torch.nn.Module):
         math_dtype=None,
         use_fallback: Optional[bool] = None,
         method: Optional[str] = None,
+        saved_activations: str = "full",
     ):
         super().__init__()
         if use_fallback:
@@ -304,7 +362,11 @@ class Linear(torch.nn.Module):
             fused = _fused_paths(paths, d.operands[1], d.operands[2])
             if fused is not None:
                 mul_ir = (int(self.transpose_in.f is not None), int(self.transpose_out.f is not None))
-                self._fused_plan = {**fused, "out_size": d.operands[2].size, "mul_ir": mul_ir}
+                self._fused_plan = {**fused, "in_size": d.operands[1].size, "out_size": d.operands[2].size, "mul_ir": mul_ir}
+        self.saved_activations = saved_activations
+        if check_saved_activations(saved_activations) and self._fused_plan is None:
+            raise ValueError("Linear(saved_activations='int8') needs multiplicities 32, 64, 96 or 128, irreps up to l = 3, at most "
+                             f"{_lib.LINEAR_MAX_PATHS} irreps and no two paths on one block of rows; got {irreps_in} -> {irreps_out}")
         try:
             self.f = SegmentedPolynomial(e.polynomial, method=self.method, math_dtype=math_dtype, name="linear")
             self._generic_error = None
@@ -316,6 +378,23 @@ class Linear(torch.nn.Module):
     def extra_repr(self) -> str:
         return (f"shared_weights={self.shared_weights}, internal_weights={self.internal_weights}, "
                 f"weight_numel={self.weight_numel}, weight_classes={self.weight_classes}")
+
+    def _forward_8_bits(self, x, weight, weight_indices):
+        if not (x.is_cuda and x.dim() == 2 and x.dtype == torch.float32 and weight.dtype == torch.float32 and weight.device == x.device
+                and x.shape[1] == self.irreps_in.dim and tuple(weight.shape) == (self.weight_classes, self.weight_numel)
+                and self.weight_classes <= _lib.LINEAR_MAX_CLASSES and x.shape[0] < 2**31):
+            raise ValueError("Linear(saved_activations='int8') needs float32 CUDA tensors x [batch, irreps_in.dim] and weight [weight_classes, "
+                             f"weight_numel] with at most {_lib.LINEAR_MAX_CLASSES} classes")
+        bounds = (0, x.shape[0])
+        if self.weight_classes > 1:
+            if weight_indices.shape[0] != x.shape[0]:
+                raise ValueError("weight_indices must have one entry per row of x")
+            bounds = class_bounds(weight_indices, self.weight_classes)
+            if bounds is None:
+                raise ValueError("Linear(saved_activations='int8') does not support non-sorted indices")
+        if torch.is_grad_enabled() and weight.requires_grad:
+            return _FusedLinear8.apply(self._fused_plan, tuple(bounds), weight, x)
+        return _FusedLinear.apply(self._fused_plan, tuple(bounds), weight, x)
 
     def forward(self, x: torch.Tensor, weight: Optional[torch.Tensor] = None, weight_indices: Optional[torch.Tensor] = None) -> torch.Tensor:
         if self.weight is not None:
@@ -329,6 +408,8 @@ class Linear(torch.nn.Module):
             input_indices[0] = weight_indices
         if weight is None:
             raise ValueError("Weights should not be None")
+        if self.saved_activations == "int8":
+            return self._forward_8_bits(x, weight, weight_indices)
         if self._fused_plan is not None and DENSE_ROUTE and x.is_cuda and x.dim() == 2 and x.dtype == torch.float32 and weight.dtype == torch.float32 \
                 and x.shape[1] == self.irreps_in.dim and weight.shape[1] == self.weight_numel and x.shape[0] < 2**31:
             if not input_indices and weight.shape[0] == 1 and x.shape[0] >= DENSE_MIN_ROWS:

@@ -453,6 +453,23 @@ int64_t cueq_b200_linear_gw_floats(const cueq_linear_args* args);
 int cueq_b200_linear_map(const cueq_linear_args* args, void* stream);
 int cueq_b200_linear_gw(const cueq_linear_args* args, void* stream);
 
+/* The layer's input kept in 8 bits for the weight gradient: per row and path x ~ step * code, code = rint(x / step), step the
+ * smallest power of two (at least 2^-126) of which 127 hold the block's largest magnitude; NaN with codes 0 where the block holds an
+ * infinity or NaN.  linear_pack writes codes and steps of all `rows` of x (args: x, ldx and the paths; w and out not read, not
+ * null); linear_gw_codes is linear_gw on step * code in place of x (args->x not read, not null).  Blocks of codes follow one another in the
+ * order of the paths, laid out as in x. */
+typedef struct {
+  int32_t struct_bytes;  /* sizeof(cueq_linear_codes)                                               */
+  int32_t reserved;
+  int64_t rows;
+  void* codes;           /* device int8 [rows, ld_codes], 16-byte aligned                           */
+  int64_t ld_codes;      /* sum of u * d over the paths or more, a multiple of 16                   */
+  void* steps;           /* device float32 [num_paths, ld_steps], 16-byte aligned                   */
+  int64_t ld_steps;      /* rows or more, a multiple of 4                                           */
+} cueq_linear_codes;
+int cueq_b200_linear_pack(const cueq_linear_args* args, const cueq_linear_codes* codes, void* stream);
+int cueq_b200_linear_gw_codes(const cueq_linear_args* args, const cueq_linear_codes* codes, void* stream);
+
 /* ---- fully connected ("uvw") tensor product: kernels around the tensor-core GEMM -----------------
  *
  * For one path of uvw,iu,jv,kw+ijk (cue.descriptors.fully_connected_tensor_product,

@@ -100,3 +100,37 @@ def test_sizes_that_a_caller_allocates():
     assert L.cueq_b200_norm_parts(C.byref(a)) % (2 * 4) == 0 and L.cueq_b200_norm_parts(C.byref(a)) <= 2 * 8 * 3
     a = _args(_lib.NORM_BRANCH, blocks=((100000, 1),))
     assert L.cueq_b200_norm_parts(C.byref(a)) == -1 and "shared memory" in L.cueq_b200_last_error().decode()
+
+
+def test_linear_refusals():
+    kw = dict(layout=cb.mul_ir, saved_activations="int8")
+    for bad in (("48x0e", "32x0e"), ("160x0e", "32x0e"), ("32x4e", "32x4e"), ("32x0e+32x0e", "32x0e")):
+        with pytest.raises(ValueError, match="int8"):
+            cb.Linear(*bad, **kw)
+    with pytest.raises(ValueError, match="saved_activations"):
+        cb.Linear("32x0e", "32x0e", saved_activations="fp8")
+    m = cb.Linear("32x0e", "32x0e", **kw)
+    with pytest.raises(ValueError, match="CUDA"):
+        m(torch.zeros(4, 32))
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(struct_bytes=4), "another block"), (dict(codes=None), "null codes"), (dict(ld_codes=112), "rows of codes"), (dict(ld_codes=136), "rows of codes"),
+    (dict(ld_steps=8), "rows of codes"), (dict(ld_steps=11), "rows of codes"), (dict(rows=8), "class bounds"), (dict(steps=8), "rows of codes"),
+])
+def test_refusals_of_the_linear_codes(change, text):
+    m = cb.Linear("32x0e+32x1o", "32x0e+32x1o", layout=cb.mul_ir, internal_weights=False, shared_weights=True)
+    a, c = _lib.LinearArgs(), _lib.LinearCodes()
+    a.x = a.w = a.out = a.parts = 16
+    a.bounds, a.parts_floats = _lib.int32_array([0, 9]), 1 << 20
+    a.num_paths, a.num_classes, a.struct_bytes = 2, 1, C.sizeof(a)
+    a.ldx = a.ldo = 128
+    for q, (wo, u, v, xo, oo, d, k) in zip(a.paths, m._fused_plan["paths"]):
+        q.u, q.v, q.d, q.x_off, q.out_off, q.w_off, q.c = u, v, d, xo, oo, wo, k
+    c.struct_bytes, c.rows, c.codes, c.ld_codes, c.steps, c.ld_steps = C.sizeof(c), 9, 16, 128, 16, 12
+    for k, v in change.items():
+        setattr(c, k, v)
+    L = _lib.lib()
+    for fn in (L.cueq_b200_linear_pack, L.cueq_b200_linear_gw_codes):
+        assert fn(C.byref(a), C.byref(c), None) != 0 and text in L.cueq_b200_last_error().decode()
+        assert fn(C.byref(a), None, None) != 0
