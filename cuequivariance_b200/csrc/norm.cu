@@ -9,7 +9,9 @@ namespace {
 using namespace cueq_norm;
 
 constexpr int kSmemPerSm = 227 * 1024, kSms = 148;
-constexpr int kStageBytes = 8192;        // rows are put together up to about this much per stage
+constexpr int kSliceValues = 1024;       // neighbouring irrep blocks are put together up to this length
+constexpr int kItemCost = 64;            // what a (row, block) costs besides its values, in values
+constexpr int kStageBytes = 4096;        // rows are put together up to about this much per stage
 
 int element_size(int dtype) { return dtype == CUEQ_F64 ? 8 : dtype == CUEQ_F32 ? 4 : 2; }
 bool gated(const cueq_norm_args* a) { return a->gate != CUEQ_NORM_GATE_NONE && (a->mode & kBranch); }
@@ -41,97 +43,147 @@ int64_t code_layout(const cueq_norm_args* a, Params* p) {
   return at;
 }
 
-// Divides the work.  A warp works alone on items of up to 256 values, two on up to 512, four on longer ones, but never more warps
-// than there are groups of 32 channels.  Thread blocks are dealt to irrep blocks by their length; with few rows a stage holds
-// fewer of them, so that they spread over the SMs.
-int make_plan(const cueq_norm_args* a, bool backward, bool bulk, Params* p, int* grid, int* smem_bytes) {
-  const bool q8 = a->codes != nullptr, gate = gated(a);
-  const int size = element_size(a->dtype), msize = a->dtype == CUEQ_F64 ? 8 : 4, stat = stats_per_item(a) * msize;
-  int64_t total_cost = 0;
-  int smem = 0, dim_total = 0, channels = 0;
+enum { kTooLong = 1, kTooLongForUnits = 2 };
+
+// Which way each tensor moves, for slices that are `whole` rows or parts of rows that start and end on 16-byte boundaries (`even`).
+void set_routes(const cueq_norm_args* a, bool backward, Params* p, bool whole, bool even) {
+  const int size = element_size(a->dtype);
+  auto route = [&](const void* q, int64_t ld, int64_t width) -> signed char {
+    if (((uintptr_t)q & 15) || (!even && !whole)) return kPlain;
+    if (whole && ld == width) return kDense;
+    return even && ld * size % 16 == 0 ? kRows : kPlain;
+  };
+  const int64_t d = p->dim_total, c = p->channels;
+  p->route[tX] = route(a->x, a->ldx, d); p->route[tY] = route(a->y, a->ldy, d); p->route[tH] = route(a->h, a->ldh, d);
+  p->route[tGo] = route(a->go, a->ldgo, d); p->route[tGn] = route(a->gn, a->ldgn, d); p->route[tG] = route(a->g, a->ldg, c);
+  p->route[tOut] = route(a->out, d, d); p->route[tNorm] = route(a->norm, d, d);
+  p->route[tDx] = route(a->dx, d, d); p->route[tDy] = route(a->dy, d, d); p->route[tDg] = route(a->dg, c, c);
+  p->route[tStats] = whole ? kDense : kRows;
+  // An operand and the result in its place have rows at one distance: dense together, or each row by itself where that is possible.
+  auto pair = [&](int in, int out) {
+    if ((p->route[in] == kDense) == (p->route[out] == kDense)) return;
+    const int t = p->route[in] == kDense ? in : out;
+    p->route[t] = even ? kRows : kPlain;
+  };
+  if (!backward) {
+    pair(tX, a->mode & kBranch ? tOut : tNorm);
+    if (a->mode == kBoth) pair(tY, tNorm);
+  } else {
+    if (a->mode == kBranch) pair(tGo, tDy);
+    if (a->mode == kNorm) pair(tGn, tDx);
+    if (a->mode == kBoth) { if (a->go) pair(tGo, tDx); pair(tGn, tDy); }
+    if (gated(a) && !a->codes) pair(tG, tDg);
+  }
+}
+
+// Lanes that issue the copies of a stage of rps rows, in or out (the larger).
+int copy_lanes(const cueq_norm_args* a, bool backward, const Params& p, int rps) {
+  const bool branch = a->mode & kBranch, norm = a->mode & kNorm, gate = gated(a), q8 = a->codes != nullptr, both = a->mode == kBoth;
+  auto lanes = [&](bool on, int t) { return !on || p.route[t] == kPlain ? 0 : p.route[t] == kDense ? 1 : rps; };
+  const int codes = q8 ? (1 + both + gate) * rps : 0;
+  int in, out;
+  if (!backward) {
+    in = lanes(true, tX) + lanes(branch, tY) + lanes(gate, tG);
+    out = lanes(branch, tOut) + lanes(norm, tNorm) + codes;
+  } else {
+    in = lanes(true, tStats) + lanes(branch && a->go, tGo) + lanes(norm, tGn) + (q8 ? codes : lanes(norm, tH) + lanes(branch, tY) + lanes(gate, tG));
+    out = lanes(norm, tDx) + lanes(branch, tDy) + lanes(gate, tDg);
+  }
+  return in > out ? in : out;
+}
+
+// Divides the work: neighbouring irrep blocks to slices of at most kSliceValues values (a longer block is a slice by itself), slices and rows to
+// warps.  A warp's share of the grid is its slice's length; with few rows a stage holds fewer of them, so that they spread over the SMs.
+// Rows that are dense but no multiple of 16 bytes come in stages of 2, 4 or 8, which are.
+int make_plan(const cueq_norm_args* a, bool backward, bool dense, Params* p, int* grid, int* smem_bytes) {
+  const bool q8 = a->codes != nullptr;
+  const int size = element_size(a->dtype), msize = a->dtype == CUEQ_F64 ? 8 : 4, stat = p->ns * msize;
+  int64_t total = 0;
+  int ns = 0;
+  bool even = true;
   for (int k = 0; k < a->num_blocks; ++k) {
     Blk& b = p->blk[k];
     b.mul = a->blocks[k].mul; b.dim = a->blocks[k].dim;
-    b.off = dim_total; b.ch = channels;
-    dim_total += b.mul * b.dim; channels += b.mul;
-    const int n = b.mul * b.dim, groups = (b.mul + 31) / 32;
-    b.wpi = n <= 256 || groups == 1 ? 1 : n <= 512 || groups == 2 ? 2 : 4;
-    auto stage = [&](int rps) { return backward ? backward_stage(a->mode, q8, gate, size, b.mul, b.dim, rps, stat).total : forward_stage(a->mode, q8, gate, size, b.mul, b.dim, rps).total; };
-    const int one = stage(1), ng = kWarps / b.wpi, head = head_bytes(msize, b.mul, backward, b.wpi);
-    int rps = kStageBytes / one;
-    rps = rps < ng ? ng : rps > 32 ? 32 : rps;
-    while (rps > 1 && head + 2 * stage(rps) > kSmemPerSm / 4) --rps;
-    b.rps = rps;
-    const int need = head + (bulk ? 2 : 1) * stage(rps);
-    smem = need > smem ? need : smem;
-    total_cost += n + 96;
+    b.off = p->dim_total; b.ch = p->channels;
+    const int n = b.mul * b.dim;
+    b.inv_n = 1.0 / n;
+    if (!ns || p->slice[ns - 1].values + n > kSliceValues) { p->slice[ns] = Slice{}; p->slice[ns].first = k; ++ns; }
+    Slice& s = p->slice[ns - 1];
+    if (s.count == 0 && (b.off * size % 16 || (gated(a) && b.ch * size % 16))) even = false;
+    ++s.count; s.values += n; s.channels += b.mul;
+    p->dim_total += n; p->channels += b.mul;
   }
-  if (smem > kSmemPerSm) return -1;
+  if (p->dim_total * size % 16 || (gated(a) && p->channels * size % 16)) even = false;
+  p->num_slices = ns; p->nb = a->num_blocks;
+  set_routes(a, backward, p, dense && ns == 1, even);
+  int unit = 1;                                          // rows after which dense rows are on a 16-byte boundary again
+  if (dense && ns == 1) while (unit < 8 && (unit * p->dim_total * size % 16 || (gated(a) && unit * p->channels * size % 16))) unit *= 2;
+  auto stage = [&](const Slice& s) { return backward ? backward_stage(*p, s, a->mode, q8, size, stat).total : forward_stage(*p, s, a->mode, q8, size).total; };
+  auto need = [&](const Slice& s, int stages) { return head_bytes(msize, s.channels, backward) + stages * stage(s); };
+  p->stages = 2;
+  for (int k = 0; k < ns; ++k) {
+    Slice& s = p->slice[k];
+    s.rps = unit;
+    if (unit > 1 && need(s, 2) > kSmemPerSm / 2) return kTooLongForUnits;
+    if (need(s, 2) > kSmemPerSm) p->stages = 1;
+    const int one = stage(s) / unit;
+    int rps = kStageBytes / (one ? one : 1) / unit * unit;
+    s.rps = rps < unit ? unit : rps > 32 ? 32 : rps;
+    while (s.rps > unit && copy_lanes(a, backward, *p, s.rps) > 32) s.rps -= unit;
+    total += s.values + kItemCost * s.count;
+  }
+  // fewer rows per stage where that lets each warp of a full GPU have some
+  int smem = 0;
+  for (int k = 0; k < ns; ++k) { const int b = need(p->slice[k], p->stages); smem = b > smem ? b : smem; }
+  *smem_bytes = smem;
+  if (smem > kSmemPerSm) return kTooLong;
   int occupancy = kSmemPerSm / (smem + 1024);
-  occupancy = occupancy < 1 ? 1 : occupancy;
-  const int most = msize == 8 ? 4 : 8;
-  occupancy = occupancy > most ? most : occupancy;
-  const int64_t ctas = (int64_t)kSms * occupancy;
+  occupancy = occupancy > warps_per_sm(msize) ? warps_per_sm(msize) : occupancy;
+  const int64_t warps = (int64_t)kSms * (occupancy < 1 ? 1 : occupancy);
   int at = 0;
   int64_t part = 0;
-  for (int k = 0; k < a->num_blocks; ++k) {
-    Blk& b = p->blk[k];
-    int64_t share = ctas * (b.mul * b.dim + 96) / total_cost;
+  for (int k = 0; k < ns; ++k) {
+    Slice& s = p->slice[k];
+    int64_t share = warps * (s.values + kItemCost * s.count) / total;
     share = share < 1 ? 1 : share;
-    const int64_t spread = a->rows / share;
-    if (b.rps > spread) b.rps = spread < 1 ? 1 : (int)spread;
-    const int64_t units = (a->rows + b.rps - 1) / b.rps;
-    b.ncta = (int)(share < units ? share : units);
-    b.cta0 = at;
-    at += b.ncta;
-    b.part = part;
-    part += (int64_t)b.ncta * b.mul;
+    const int64_t spread = a->rows / share / unit * unit;
+    if (s.rps > spread) s.rps = spread < unit ? unit : (int)spread;
+    const int64_t units = (a->rows + s.rps - 1) / s.rps;
+    s.ncta = (int)(share < units ? share : units);
+    s.cta0 = at;
+    at += s.ncta;
+    s.part = part;
+    part += (int64_t)s.ncta * s.channels;
   }
-  p->nb = a->num_blocks; p->dim_total = dim_total; p->channels = channels;
   p->parts_len = part;
   *grid = at;
-  *smem_bytes = smem;
   return 0;
 }
 
-bool aligned(const void* q, int64_t ld_bytes) { return !q || (((uintptr_t)q | (uintptr_t)ld_bytes) & 15) == 0; }
-
-// Bulk copies want 16-byte boundaries and lengths.
-bool bulk_ok(const cueq_norm_args* a) {
-  const int size = element_size(a->dtype);
-  int64_t dim = 0, channels = 0;
-  for (int k = 0; k < a->num_blocks; ++k) {
-    const int64_t n = (int64_t)a->blocks[k].mul * a->blocks[k].dim;
-    if (n * size % 16 || (gated(a) && a->blocks[k].mul * size % 16)) return false;
-    dim += n; channels += a->blocks[k].mul;
-  }
-  const void* operands[] = {a->x, a->y, a->g, a->h, a->go, a->gn};
-  const int64_t lds[] = {a->ldx, a->ldy, a->ldg, a->ldh, a->ldgo, a->ldgn};
-  for (int k = 0; k < 6; ++k) if (!aligned(operands[k], lds[k] * size)) return false;
-  const void* rows[] = {a->out, a->norm, a->dx, a->dy};
-  for (const void* q : rows) if (!aligned(q, dim * size)) return false;
-  return aligned(a->dg, channels * size);
-}
-
 int fill(const cueq_norm_args* a, bool backward, Params* p, int* grid, int* smem) {
-  std::memset(p, 0, sizeof(*p));
   if (int rc = check(a)) return rc;
-  p->bulk = bulk_ok(a);
-  int rc = make_plan(a, backward, p->bulk, p, grid, smem);
-  if (rc && p->bulk) { p->bulk = 0; rc = make_plan(a, backward, false, p, grid, smem); }   // one stage at a time
+  int rc = kTooLongForUnits;
+  for (int dense = 1; dense >= 0 && rc == kTooLongForUnits; --dense) {
+    std::memset(p, 0, sizeof(*p));
+    p->ns = stats_per_item(a);
+    p->gate = a->mode & kBranch ? a->gate : CUEQ_NORM_GATE_NONE;
+    p->go = a->go;
+    code_layout(a, p);
+    rc = make_plan(a, backward, dense, p, grid, smem);
+  }
   if (rc) return cueq::fail("norm: an irrep block does not fit into shared memory (%d bytes of %d)", *smem, kSmemPerSm);
   return 0;
 }
 
-// dscale, dweight: the thread blocks' sums of a channel, in order
+// dscale, dweight: the warps' sums of a channel, in order
 struct SumParams {
   const void* parts;
   int64_t parts_len;
   void* out[2];
-  int nb, channels, dtype;
-  struct { int mul, ch, ncta; int64_t part; } blk[kMaxBlocks];
+  int num_slices, channels, dtype;
+  struct { int channels, ch, ncta; int64_t part; } slice[kMaxBlocks];
 };
-constexpr int kSumRows = 16;
+constexpr int kSumRows = 32;
 template <class M>
 __global__ void __launch_bounds__(32 * kSumRows) sum_kernel(const __grid_constant__ SumParams p) {
   __shared__ M partial[kSumRows][33];
@@ -140,10 +192,10 @@ __global__ void __launch_bounds__(32 * kSumRows) sum_kernel(const __grid_constan
   M v = M(0);
   if (ch < p.channels && p.out[which]) {
     int k = 0;
-    while (k + 1 < p.nb && ch >= p.blk[k + 1].ch) ++k;
-    const M* src = reinterpret_cast<const M*>(p.parts) + which * p.parts_len + p.blk[k].part + (ch - p.blk[k].ch);
+    while (k + 1 < p.num_slices && ch >= p.slice[k + 1].ch) ++k;
+    const M* src = reinterpret_cast<const M*>(p.parts) + which * p.parts_len + p.slice[k].part + (ch - p.slice[k].ch);
 #pragma unroll 8
-    for (int j = threadIdx.y; j < p.blk[k].ncta; j += kSumRows) v += src[(int64_t)j * p.blk[k].mul];
+    for (int j = threadIdx.y; j < p.slice[k].ncta; j += kSumRows) v += src[(int64_t)j * p.slice[k].channels];
   }
   partial[threadIdx.y][threadIdx.x] = v;
   __syncthreads();
@@ -159,12 +211,12 @@ __global__ void __launch_bounds__(32 * kSumRows) sum_kernel(const __grid_constan
   }
 }
 
-Kernel pick_kernel(int dtype, int mode, bool q8, bool backward) {
+Kernel pick_kernel(int dtype, int mode, bool q8, bool mul_ir, bool backward) {
   switch (dtype) {
-    case CUEQ_F32: return pick_f32(mode, q8, backward);
-    case CUEQ_F64: return pick_f64(mode, q8, backward);
-    case CUEQ_BF16: return pick_bf16(mode, q8, backward);
-    default: return pick_f16(mode, q8, backward);
+    case CUEQ_F32: return pick_f32(mode, q8, mul_ir, backward);
+    case CUEQ_F64: return pick_f64(mode, q8, mul_ir, backward);
+    case CUEQ_BF16: return pick_bf16(mode, q8, mul_ir, backward);
+    default: return pick_f16(mode, q8, mul_ir, backward);
   }
 }
 
@@ -200,19 +252,17 @@ int launch(const cueq_norm_args* a, bool backward, void* stream) {
   p.codes = (signed char*)a->codes; p.ldc = a->ld_codes;
   p.stats = a->stats; p.parts = a->parts;
   p.rows = a->rows; p.eps = a->eps; p.status = (int*)a->status;
-  p.ns = stats_per_item(a);
   p.pdtype = a->param_dtype; p.mul_ir = a->mul_ir;
-  p.gate = branch ? a->gate : CUEQ_NORM_GATE_NONE;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (a->rows) {
-    const Kernel kernel = pick_kernel(a->dtype, a->mode, q8, backward);
-    static cueq::PerDeviceFlag configured[4][3][2][2];
-    cueq::PerDeviceFlag& flag = configured[a->dtype][a->mode - 1][q8][backward];
+    const Kernel kernel = pick_kernel(a->dtype, a->mode, q8, a->mul_ir, backward);
+    static cueq::PerDeviceFlag configured[4][3][2][2][2];
+    cueq::PerDeviceFlag& flag = configured[a->dtype][a->mode - 1][q8][a->mul_ir != 0][backward];
     if (!flag.get()) {
       CUEQ_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemPerSm));
       flag.set();
     }
-    kernel<<<grid, kThreads, smem, st>>>(p);
+    kernel<<<grid, 32, smem, st>>>(p);
     CUEQ_CUDA_OK(cudaGetLastError());
   }
   if (!backward) return 0;
@@ -222,8 +272,11 @@ int launch(const cueq_norm_args* a, bool backward, void* stream) {
   s.out[0] = branch ? a->dscale : nullptr;
   s.out[1] = norm ? a->dweight : nullptr;
   if (!s.out[0] && !s.out[1]) return 0;
-  s.nb = p.nb; s.channels = p.channels; s.dtype = a->param_dtype;
-  for (int k = 0; k < p.nb; ++k) { s.blk[k].mul = p.blk[k].mul; s.blk[k].ch = p.blk[k].ch; s.blk[k].ncta = a->rows ? p.blk[k].ncta : 0; s.blk[k].part = p.blk[k].part; }
+  s.num_slices = p.num_slices; s.channels = p.channels; s.dtype = a->param_dtype;
+  for (int k = 0; k < p.num_slices; ++k) {
+    const Slice& q = p.slice[k];
+    s.slice[k].channels = q.channels; s.slice[k].ch = p.blk[q.first].ch; s.slice[k].ncta = a->rows ? q.ncta : 0; s.slice[k].part = q.part;
+  }
   const dim3 g((p.channels + 31) / 32, 2), t(32, kSumRows);
   if (a->dtype == CUEQ_F64) sum_kernel<double><<<g, t, 0, st>>>(s);
   else sum_kernel<float><<<g, t, 0, st>>>(s);

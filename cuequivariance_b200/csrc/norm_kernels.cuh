@@ -11,11 +11,12 @@
 // (r c and no r^3: that leaves the range of 32 bits for blocks of 1e13 or 1e-13)
 // and the same with (w, gn, h) for (a, go, y) for the norm; behind a branch its result is added to go first.
 //
-// What bounds them: HBM.  Every value is read once and written once.  A thread block belongs to one irrep block and a range of
-// rows.  It brings the rows' items into shared memory by bulk copies, the next stage while it works on this one; a thread owns
-// channels and reads their components there at a stride of dim words (odd: no bank conflicts; neighbouring words in ir_mul),
-// so neither layout needs a transposition and sums over components need no other thread.  Results replace the operands in
-// shared memory and leave by bulk copies.  A warp, two or four work on one item, by its size (see the plan in norm.cu).
+// What bounds them: HBM.  Every value is read once and written once.  A thread block is one warp.  It belongs to a slice of the
+// irrep blocks (neighbours of 1,024 values together, one block if that is longer) and to a range of rows, and brings the slice's part of a few rows
+// into shared memory by bulk copies, the next stage while it works on this one: no barrier between warps anywhere, and 7 to 30 stages
+// under way per SM.  A lane owns channels and reads their components in shared memory at a stride of dim words (odd: no bank conflicts;
+// neighbouring words in ir_mul), so neither layout needs a transposition and sums over components need no other lane.  Results
+// replace the operands in shared memory and leave by bulk copies.
 //
 // Sums, statistics and all arithmetic are in 32 bits for 16- and 32-bit data, in 64 for 64-bit data; results are rounded once.
 //
@@ -32,16 +33,26 @@ using cueq_tc::bar_init;
 using cueq_tc::bar_wait;
 using cueq_tc::s32;
 
-constexpr int kThreads = 128, kWarps = 4;
 constexpr int kMaxBlocks = CUEQ_NORM_MAX_BLOCKS;
+// warps of an SM that its registers hold
+__host__ __device__ constexpr int warps_per_sm(int msize) { return msize == 8 ? 8 : 16; }
 enum Mode { kBranch = 1, kNorm = 2, kBoth = 3 };
 
 struct Blk {
   int mul, dim, off, ch;             // off, ch: first element of the block in a row of features, first channel
+  double inv_n;                      // 1 / (mul dim)
   int code, gcode, hcode;            // first byte in a row of codes: of y (or x, norm alone), of the gates, of h
-  int cta0, ncta, rps, wpi;          // thread blocks, rows per stage, warps per item
+};
+struct Slice {
+  int first, count;                  // blocks
+  int values, channels;              // their elements and channels
+  int cta0, ncta, rps;               // thread blocks, rows per stage
   int64_t part;                      // first partial sum
 };
+// How rows of an operand move.  kRows: a bulk copy per row; kDense: rows follow one another without a gap, one bulk copy per stage;
+// kPlain: element by element, where addresses or lengths are not multiples of 16 bytes.
+enum Route { kPlain, kRows, kDense };
+enum Tensor { tX, tY, tG, tH, tGo, tGn, tOut, tNorm, tDx, tDy, tDg, tCa, tCg, tCh, tStats, kTensors };
 
 struct Params {
   const void *x, *y, *g, *h, *go, *gn;
@@ -57,53 +68,74 @@ struct Params {
   int64_t rows;
   double eps;
   int* status;
-  int nb, dim_total, channels, ns;   // ns: statistics per (row, block)
-  int pdtype, gate, mul_ir, bulk;
+  int nb, ns, dim_total, channels;   // ns: statistics per (row, block)
+  int num_slices, stages;            // stages: 2, or 1 where two do not fit into shared memory
+  int pdtype, gate, mul_ir;
+  signed char route[kTensors];
   Blk blk[kMaxBlocks];
+  Slice slice[kMaxBlocks];
 };
 
 __host__ __device__ constexpr int pad16(int bytes) { return (bytes + 15) & ~15; }
+__host__ __device__ inline int code_bytes(const Params& p, const Slice& s) {
+  int n = 0;
+  for (int k = s.first; k < s.first + s.count; ++k) n += pad16(p.blk[k].mul * p.blk[k].dim);
+  return n;
+}
+__host__ __device__ inline int gate_code_bytes(const Params& p, const Slice& s) {
+  int n = 0;
+  for (int k = s.first; k < s.first + s.count; ++k) n += pad16(p.blk[k].mul);
+  return n;
+}
 
-// Byte offsets of a stage's regions.  A region holds one item per row, 16 bytes apart or more.
-struct Stage { int a, b, c, d, g, dg, ca, cg, cb, st, total; };
+// Regions of a stage: byte offset, distance and length of the rows.
+struct Region { int at, pitch, bytes; };
+struct Stage { Region a, b, c, d, g, dg, ca, cg, ch, st; int total; };
 
-// forward: a = x, b = y, g = gates, ca / cg / cb = codes of y (x), gates, h
-__host__ __device__ inline Stage forward_stage(int mode, bool q8, bool gated, int size, int mul, int dim, int rps) {
-  Stage s{};
-  const int item = pad16(mul * dim * size), gate = pad16(mul * size), code = pad16(mul * dim), gcode = pad16(mul);
+__host__ __device__ inline Region region(bool on, int bytes, bool dense, int rps, int& at) {
+  const Region r{at, dense ? bytes : pad16(bytes), bytes};
+  if (on) at += pad16(r.pitch * rps);
+  return r;
+}
+// An operand and the result that replaces it share rows: without gaps only if both are.
+__host__ __device__ inline bool both_dense(const Params& p, int in, int out) { return p.route[in] == kDense && p.route[out] == kDense; }
+
+// forward: a = x (then out, or norm alone), b = y (then norm), g = gates, ca / cg / ch = codes of y (x), gates, out
+__host__ __device__ inline Stage forward_stage(const Params& p, const Slice& s, int mode, bool q8, int size) {
+  Stage t{};
+  const bool branch = mode & kBranch, gated = branch && p.gate != CUEQ_NORM_GATE_NONE;
+  const int item = s.values * size, rps = s.rps;
   int at = 0;
-  auto put = [&](bool on, int bytes) { const int o = at; if (on) at += bytes * rps; return o; };
-  s.a = put(true, item);
-  s.b = put(mode & kBranch, item);
-  s.g = put((mode & kBranch) && gated, gate);
-  s.ca = put(q8, code);
-  s.cg = put(q8 && (mode & kBranch) && gated, gcode);
-  s.cb = put(q8 && mode == kBoth, code);
-  s.total = at;
-  return s;
+  t.a = region(true, item, both_dense(p, tX, branch ? tOut : tNorm), rps, at);
+  t.b = region(branch, item, mode == kBoth ? both_dense(p, tY, tNorm) : p.route[tY] == kDense, rps, at);
+  t.g = region(gated, s.channels * size, p.route[tG] == kDense, rps, at);
+  t.ca = region(q8, code_bytes(p, s), false, rps, at);
+  t.cg = region(q8 && gated, gate_code_bytes(p, s), false, rps, at);
+  t.ch = region(q8 && mode == kBoth, code_bytes(p, s), false, rps, at);
+  t.total = at;
+  return t;
 }
-// backward: a = go, b = gn, c = h, d = y, g = gates, dg = their gradient (over g where that is not in codes), st = statistics
-__host__ __device__ inline Stage backward_stage(int mode, bool q8, bool gated, int size, int mul, int dim, int rps, int stat_bytes) {
-  Stage s{};
-  const int item = pad16(mul * dim * size), gate = pad16(mul * size), code = pad16(mul * dim), gcode = pad16(mul);
+// backward: a = go (then dx behind a branch with a norm, dy behind one without), b = gn (then dy, or dx for the norm alone), c = h,
+// d = y, g = gates, dg = their gradient (over g where that is not in codes), st = statistics
+__host__ __device__ inline Stage backward_stage(const Params& p, const Slice& s, int mode, bool q8, int size, int stat_bytes) {
+  Stage t{};
+  const bool branch = mode & kBranch, norm = mode & kNorm, gated = branch && p.gate != CUEQ_NORM_GATE_NONE;
+  const int item = s.values * size, rps = s.rps, kept = q8 ? code_bytes(p, s) : item;
   int at = 0;
-  auto put = [&](bool on, int bytes) { const int o = at; if (on) at += bytes * rps; return o; };
-  s.a = put(mode & kBranch, item);
-  s.b = put(mode & kNorm, item);
-  s.c = put(mode & kNorm, q8 ? code : item);
-  s.d = put(mode & kBranch, q8 ? code : item);
-  const bool gates = (mode & kBranch) && gated;
-  s.g = put(gates, q8 ? gcode : gate);
-  s.dg = q8 ? put(gates, gate) : s.g;
-  s.st = put(true, stat_bytes);
-  s.total = at;
-  return s;
+  t.a = region(branch, item, mode == kBoth ? p.route[tDx] == kDense && (!p.go || p.route[tGo] == kDense) : both_dense(p, tGo, tDy), rps, at);
+  t.b = region(norm, item, both_dense(p, tGn, mode == kBoth ? tDy : tDx), rps, at);
+  t.c = region(norm, kept, !q8 && p.route[tH] == kDense, rps, at);
+  t.d = region(branch, kept, !q8 && p.route[tY] == kDense, rps, at);
+  t.g = region(gated, q8 ? gate_code_bytes(p, s) : s.channels * size, !q8 && both_dense(p, tG, tDg), rps, at);
+  t.dg = t.g;
+  if (q8) t.dg = region(gated, s.channels * size, p.route[tDg] == kDense, rps, at);
+  t.st = region(true, s.count * stat_bytes, p.route[tStats] == kDense, rps, at);
+  t.total = at;
+  return t;
 }
-// in front of the stages: 2 barriers, room of the reductions, s and w, and (backward) sums of both per group of warps
-constexpr int kRed = 16, kRedBytes = 2 * kWarps * 16;
-__host__ __device__ inline int head_bytes(int msize, int mul, bool backward, int wpi) {
-  return (kRed + kRedBytes + msize * mul * (2 + (backward ? 2 * (kWarps / wpi) : 0)) + 127) & ~127;
-}
+// in front of the stages: 2 barriers and the tensors' moves; per channel s, w, s act(g) of the row at work, and (backward) the sums of both gradients
+constexpr int kMoves = 11, kMoveBytes = 40, kBars = 16 + kMoves * kMoveBytes + 8;
+__host__ __device__ inline int head_bytes(int msize, int channels, bool backward) { return (kBars + msize * channels * (backward ? 5 : 3) + 127) & ~127; }
 
 // ---- conversions ----------------------------------------------------------------------------------------------------
 template <class M> __device__ __forceinline__ M to(float v) { return (M)v; }
@@ -118,17 +150,19 @@ template <> __device__ __forceinline__ __nv_bfloat16 from<__nv_bfloat16>(float v
 template <> __device__ __forceinline__ __half from<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ double from<double>(double v) { return v; }
 
-__device__ __forceinline__ float inverse_sqrt(float v) { return 1.0f / sqrtf(v); }
+__device__ __forceinline__ float inverse_sqrt(float v) { return rsqrtf(v); }
 __device__ __forceinline__ double inverse_sqrt(double v) { return 1.0 / sqrt(v); }
 __device__ __forceinline__ float exponential(float v) { return expf(v); }
 __device__ __forceinline__ double exponential(double v) { return exp(v); }
+__device__ __forceinline__ float reciprocal(float v) { return __fdividef(1.0f, v); }   // 0 from 2^126 on
+__device__ __forceinline__ double reciprocal(double v) { return 1.0 / v; }
 __device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }   // ordered as |v|, NaN above all
 __device__ __forceinline__ unsigned magnitude(double) { return 0u; }                                  // 64-bit data are not kept in codes
 
 template <class M>
 __device__ __forceinline__ void activation(int gate, M g, M& v, M& dv) {
   if (gate == CUEQ_NORM_GATE_NONE) { v = M(1); dv = M(0); return; }
-  const M e = M(1) / (M(1) + exponential(-g));
+  const M e = reciprocal(M(1) + exponential(-g));
   if (gate == CUEQ_NORM_GATE_SIGMOID) { v = e; dv = e * (M(1) - e); }
   else { v = g * e; dv = e * (M(1) + g * (M(1) - e)); }
 }
@@ -137,105 +171,75 @@ using cueq::code_step;
 using cueq::to_code;
 __device__ __forceinline__ signed char to_code(double, float) { return 0; }
 
-// ---- a thread block's view of its work --------------------------------------------------------------------------------
+// ---- one (row, irrep block) ---------------------------------------------------------------------------------------------
 template <class M>
 struct View {
-  M *s, *w, *acc_s, *acc_w;          // parameters and this group's sums, per channel
-  unsigned char* red;
-  unsigned red_at;
-  int mul, dim, su, si;              // strides of a channel and a component inside an item
-  int n;                             // values of an item
-  int wpi, group, lane, warp_in, tg, gt;   // warps per item; this thread's group, its place in it, the group's threads
-  int gate, gated;
+  M *s, *w, *a, *acc_s, *acc_w;      // parameters, s act(g), sums; per channel of the block
+  int mul, dim, lane, gate, gated;
   M inv_n, eps;
 };
 
-// sum of v and maxima of a, b over the threads that share an item
-template <class M>
-__device__ __forceinline__ void reduce(View<M>& c, M& v, unsigned& a, unsigned& b) {
-  v = cueq::warp_sum(v);
-  a = __reduce_max_sync(0xffffffffu, a);
-  b = __reduce_max_sync(0xffffffffu, b);
-  if (c.wpi == 1) return;
-  // two buffers in turn: a thread that writes the third time has passed the second barrier, so all have read the first
-  unsigned char* buf = c.red + (c.red_at & 1) * (kWarps * 16);
-  ++c.red_at;
-  unsigned char* mine = buf + (c.group * c.wpi + c.warp_in) * 16;
-  if (c.lane == 0) {
-    *reinterpret_cast<M*>(mine) = v;
-    reinterpret_cast<unsigned*>(mine)[2] = a;
-    reinterpret_cast<unsigned*>(mine)[3] = b;
-  }
-  if (c.wpi == 4) asm volatile("bar.sync 1, 128;\n" ::: "memory");
-  else if (c.group == 0) asm volatile("bar.sync 1, 64;\n" ::: "memory");
-  else asm volatile("bar.sync 2, 64;\n" ::: "memory");
-  const unsigned char* all = buf + c.group * c.wpi * 16;
-  v = M(0);
-  for (int k = 0; k < c.wpi; ++k) {
-    v += *reinterpret_cast<const M*>(all + k * 16);
-    a = max(a, reinterpret_cast<const unsigned*>(all + k * 16)[2]);
-    b = max(b, reinterpret_cast<const unsigned*>(all + k * 16)[3]);
-  }
-}
-template <class M>
-__device__ __forceinline__ M reduce(View<M>& c, M v) {
-  unsigned a = 0, b = 0;
-  reduce(c, v, a, b);
-  return v;
-}
+// channel u, component i: DIM 0 is a dimension known at run time only
+template <int DIM, bool MUL_IR>
+__device__ __forceinline__ int place(int u, int i, int mul, int dim) { return MUL_IR ? u * (DIM ? DIM : dim) + i : i * mul + u; }
+// how many channels a lane takes at a time
+template <int DIM> constexpr int kUnrolled = DIM == 1 ? 4 : DIM == 3 ? 2 : 1;
+#define CUEQ_CHANNELS _Pragma("unroll (kUnrolled<DIM>)") for (int u = c.lane; u < c.mul; u += 32)
+#define CUEQ_COMPONENTS _Pragma("unroll") for (int i = 0; i < (DIM ? DIM : c.dim); ++i)
+#define CUEQ_AT place<DIM, MUL_IR>(u, i, c.mul, c.dim)
 
-// ---- forward of one item ------------------------------------------------------------------------------------------------
-template <class T, class M, int MODE, bool Q8, int DIM>
-__device__ __forceinline__ void forward_item(View<M>& c, T* x, T* y, const T* g, signed char* ca, signed char* cg, signed char* cb, M* stats) {
-  const int dim = DIM ? DIM : c.dim;
-  T* t = (MODE & kBranch) ? y : x;                       // what the first statistic is of
+template <class T, class M, int MODE, bool Q8, int DIM, bool MUL_IR>
+__device__ __forceinline__ void forward_item(const View<M>& c, T* __restrict__ x, T* __restrict__ y, const T* __restrict__ g, signed char* __restrict__ ca,
+                                             signed char* __restrict__ cg, signed char* __restrict__ ch, M* __restrict__ stats) {
+  const M *__restrict__ cs = c.s, *__restrict__ cw = c.w;
+  M* __restrict__ cc = c.a;
+  constexpr bool kHasBranch = (MODE & kBranch) != 0;
+  const T* t = kHasBranch ? y : x;                       // what the first statistic is of
   M sum = M(0);
   unsigned top = 0, gtop = 0;
-  for (int u = c.tg; u < c.mul; u += c.gt) {
-    const T* p = t + u * c.su;
-#pragma unroll
-    for (int i = 0; i < dim; ++i) {
-      const M v = to<M>(p[i * c.si]);
+  CUEQ_CHANNELS {
+    CUEQ_COMPONENTS {
+      const M v = to<M>(t[CUEQ_AT]);
       sum += v * v;
       if (Q8) top = max(top, magnitude(v));
     }
-    if (Q8 && (MODE & kBranch) && c.gated) gtop = max(gtop, magnitude(to<M>(g[u])));
+    if (Q8 && kHasBranch && c.gated) gtop = max(gtop, magnitude(to<M>(g[u])));
   }
-  reduce(c, sum, top, gtop);
+  sum = cueq::warp_sum(sum);
   const M r = inverse_sqrt(sum * c.inv_n + c.eps);
   float step = 0.f, inv = 0.f, gstep = 0.f, ginv = 0.f;
   if (Q8) {
-    code_step(top, step, inv);
-    if ((MODE & kBranch) && c.gated) code_step(gtop, gstep, ginv);
+    code_step(__reduce_max_sync(0xffffffffu, top), step, inv);
+    if (kHasBranch && c.gated) code_step(__reduce_max_sync(0xffffffffu, gtop), gstep, ginv);
   }
   if (MODE == kNorm) {
-    for (int u = c.tg; u < c.mul; u += c.gt) {
-      T* p = x + u * c.su;
-      const M a = c.w[u] * r;
-#pragma unroll
-      for (int i = 0; i < dim; ++i) {
-        const M v = to<M>(p[i * c.si]);
-        if (Q8) ca[u * c.su + i * c.si] = to_code(v, inv);
-        p[i * c.si] = from<T>(a * v);
+    CUEQ_CHANNELS {
+      const M a = cw[u] * r;
+      CUEQ_COMPONENTS {
+        const M v = to<M>(x[CUEQ_AT]);
+        if (Q8) ca[CUEQ_AT] = to_code(v, inv);
+        x[CUEQ_AT] = from<T>(a * v);
       }
     }
-    if (stats && c.tg == 0) { stats[0] = r; stats[2] = M(step); }
+    if (stats && c.lane == 0) { stats[0] = r; stats[2] = M(step); }
     return;
   }
   M hsum = M(0);
-  unsigned htop = 0, none = 0;
-  for (int u = c.tg; u < c.mul; u += c.gt) {
-    M v, dv;
-    activation(c.gate, c.gated ? to<M>(g[u]) : M(0), v, dv);
-    const M a = c.s[u] * v * r;
-    T *px = x + u * c.su, *py = y + u * c.su;
-    if (Q8 && c.gated) cg[u] = to_code(to<M>(g[u]), ginv);
-#pragma unroll
-    for (int i = 0; i < dim; ++i) {
-      const M yv = to<M>(py[i * c.si]);
-      const M h = to<M>(px[i * c.si]) + a * yv;
-      if (Q8) ca[u * c.su + i * c.si] = to_code(yv, inv);
-      if (MODE == kBranch) px[i * c.si] = from<T>(h);
+  unsigned htop = 0;
+  CUEQ_CHANNELS {
+    M v = M(1), dv;
+    if (c.gated) {
+      const M gate = to<M>(g[u]);
+      activation(c.gate, gate, v, dv);
+      if (Q8) cg[u] = to_code(gate, ginv);
+    }
+    const M a = cs[u] * v * r;
+    if (MODE == kBoth) cc[u] = a;
+    CUEQ_COMPONENTS {
+      const M yv = to<M>(y[CUEQ_AT]);
+      const M h = to<M>(x[CUEQ_AT]) + a * yv;
+      if (Q8) ca[CUEQ_AT] = to_code(yv, inv);
+      if (MODE == kBranch) x[CUEQ_AT] = from<T>(h);
       else {
         hsum += h * h;
         if (Q8) htop = max(htop, magnitude(h));
@@ -245,105 +249,263 @@ __device__ __forceinline__ void forward_item(View<M>& c, T* x, T* y, const T* g,
   M rh = M(0);
   float hstep = 0.f, hinv = 0.f;
   if (MODE == kBoth) {
-    reduce(c, hsum, htop, none);
+    hsum = cueq::warp_sum(hsum);
     rh = inverse_sqrt(hsum * c.inv_n + c.eps);
-    if (Q8) code_step(htop, hstep, hinv);
+    if (Q8) code_step(__reduce_max_sync(0xffffffffu, htop), hstep, hinv);
     // h once more from x and y: kept in 16 bits in between, n would be rounded twice
-    for (int u = c.tg; u < c.mul; u += c.gt) {
-      M v, dv;
-      activation(c.gate, c.gated ? to<M>(g[u]) : M(0), v, dv);
-      const M a = c.s[u] * v * r, b = c.w[u] * rh;
-      T *px = x + u * c.su, *py = y + u * c.su;
-#pragma unroll
-      for (int i = 0; i < dim; ++i) {
-        const M h = to<M>(px[i * c.si]) + a * to<M>(py[i * c.si]);
-        if (Q8) cb[u * c.su + i * c.si] = to_code(h, hinv);
-        px[i * c.si] = from<T>(h);
-        py[i * c.si] = from<T>(b * h);
+    CUEQ_CHANNELS {
+      const M a = cc[u], b = cw[u] * rh;
+      CUEQ_COMPONENTS {
+        const M h = to<M>(x[CUEQ_AT]) + a * to<M>(y[CUEQ_AT]);
+        if (Q8) ch[CUEQ_AT] = to_code(h, hinv);
+        x[CUEQ_AT] = from<T>(h);
+        y[CUEQ_AT] = from<T>(b * h);
       }
     }
   }
-  if (stats && c.tg == 0) {
+  if (stats && c.lane == 0) {
     stats[0] = r; stats[1] = rh; stats[2] = M(step); stats[3] = M(gstep);
     if (Q8 && MODE == kBoth) stats[4] = M(hstep);
   }
 }
 
-// ---- backward of one item -----------------------------------------------------------------------------------------------
-// go becomes dx behind a branch with a norm, dy behind one without; gn becomes dy or, norm alone, dx; dg the gates' gradient.
-// K: type of what was kept (T or codes).
-template <class T, class M, class K, int MODE, bool Q8, int DIM>
-__device__ __forceinline__ void backward_item(View<M>& c, T* go, T* gn, const K* h, const K* y, const K* g, T* dg, const M* stats, bool has_go) {
-  const int dim = DIM ? DIM : c.dim;
+// K: type of what was kept (T or codes).  r (r c) stays in range: r^2 <= 1 / eps, and r >= 1e-19 while the sum of squares is finite.
+template <class T, class M, class K, int MODE, bool Q8, int DIM, bool MUL_IR>
+__device__ __forceinline__ void backward_item(const View<M>& c, T* __restrict__ go, T* __restrict__ gn, const K* __restrict__ h, const K* __restrict__ y, const K* g, T* dg,
+                                              const M* __restrict__ stats, bool has_go) {
+  const M *__restrict__ cs = c.s, *__restrict__ cw = c.w;
+  M *__restrict__ cc = c.a, *__restrict__ acc_s = c.acc_s, *__restrict__ acc_w = c.acc_w;
   M rh = M(0), qh = M(0);
   if (MODE & kNorm) {
     rh = stats[MODE == kBoth ? 1 : 0];
     const M step = Q8 ? stats[MODE == kBoth ? 4 : 2] : M(1);
+    const M rs = rh * step;
     M dot = M(0);
-    for (int u = c.tg; u < c.mul; u += c.gt) {
+    CUEQ_CHANNELS {
       M p = M(0);
-#pragma unroll
-      for (int i = 0; i < dim; ++i) p += to<M>(gn[u * c.su + i * c.si]) * to<M>(h[u * c.su + i * c.si]);
-      p *= step;
-      c.acc_w[u] += rh * p;
-      dot += c.w[u] * p;
+      CUEQ_COMPONENTS p += to<M>(gn[CUEQ_AT]) * to<M>(h[CUEQ_AT]);
+      p *= rs;
+      acc_w[u] += p;
+      dot += cw[u] * p;
     }
-    dot = reduce(c, dot);
-    qh = rh * (rh * c.inv_n * dot) * step;
+    qh = rh * (rh * (c.inv_n * cueq::warp_sum(dot))) * step;
     if (MODE == kNorm) {
-      for (int u = c.tg; u < c.mul; u += c.gt) {
-        const M a = c.w[u];
-#pragma unroll
-        for (int i = 0; i < dim; ++i) {
-          const int e = u * c.su + i * c.si;
-          gn[e] = from<T>(rh * (a * to<M>(gn[e]) - qh * to<M>(h[e])));
-        }
+      CUEQ_CHANNELS {
+        const M a = cw[u] * rh;
+        CUEQ_COMPONENTS gn[CUEQ_AT] = from<T>(a * to<M>(gn[CUEQ_AT]) - qh * to<M>(h[CUEQ_AT]));
       }
       return;
     }
   }
-  const M r = stats[0];
-  const M step = Q8 ? stats[2] : M(1), gstep = Q8 ? stats[3] : M(1);
+  // in 32 and 64 bits what reaches h is put down once, over go; in 16 bits it is computed twice, so that dy is rounded once
+  constexpr bool kPut = MODE == kBoth && sizeof(T) == sizeof(M);
+  const M r = stats[0], step = Q8 ? stats[2] : M(1), gstep = Q8 ? stats[3] : M(1), rs = r * step;
   M dot = M(0);
-  for (int u = c.tg; u < c.mul; u += c.gt) {
-    M v, dv, p = M(0);
-    activation(c.gate, c.gated ? to<M>(g[u]) * gstep : M(0), v, dv);
-    const M b = MODE == kBoth ? c.w[u] : M(0);
-#pragma unroll
-    for (int i = 0; i < dim; ++i) {
-      const int e = u * c.su + i * c.si;
-      M o = MODE == kBranch || has_go ? to<M>(go[e]) : M(0);
-      if (MODE == kBoth) o += rh * (b * to<M>(gn[e]) - qh * to<M>(h[e]));
-      p += o * to<M>(y[e]);
+  CUEQ_CHANNELS {
+    M v = M(1), dv = M(0), p = M(0);
+    if (c.gated) activation(c.gate, to<M>(g[u]) * gstep, v, dv);
+    const M b = MODE == kBoth ? cw[u] * rh : M(0), s = cs[u];
+    CUEQ_COMPONENTS {
+      M o = MODE == kBranch || has_go ? to<M>(go[CUEQ_AT]) : M(0);
+      if (MODE == kBoth) o += b * to<M>(gn[CUEQ_AT]) - qh * to<M>(h[CUEQ_AT]);
+      if (kPut) go[CUEQ_AT] = from<T>(o);
+      p += o * to<M>(y[CUEQ_AT]);
     }
-    p *= step;
-    const M s = c.s[u];
-    c.acc_s[u] += v * r * p;
-    dot += s * v * p;
-    if (c.gated && !Q8) continue;                        // g is read once more below, before dg replaces it
-    if (c.gated) dg[u] = from<T>(s * dv * r * p);
+    p *= rs;
+    const M a = s * v;
+    cc[u] = a * r;
+    acc_s[u] += v * p;
+    dot += a * p;
+    if (c.gated) dg[u] = from<T>(s * dv * p);            // may lie over g[u]
   }
-  dot = reduce(c, dot);
-  const M q = r * (r * c.inv_n * dot) * step;
-  for (int u = c.tg; u < c.mul; u += c.gt) {
-    M v, dv, p = M(0);
-    activation(c.gate, c.gated ? to<M>(g[u]) * gstep : M(0), v, dv);
-    const M a = c.s[u] * v, b = MODE == kBoth ? c.w[u] : M(0);
-#pragma unroll
-    for (int i = 0; i < dim; ++i) {
-      const int e = u * c.su + i * c.si;
-      M o = MODE == kBranch || has_go ? to<M>(go[e]) : M(0);
-      if (MODE == kBoth) o += rh * (b * to<M>(gn[e]) - qh * to<M>(h[e]));
-      const M yv = to<M>(y[e]);
-      if (!Q8) p += o * yv;
-      const T dy = from<T>(r * (a * o - q * yv));
-      if (MODE == kBoth) { go[e] = from<T>(o); gn[e] = dy; } else go[e] = dy;
+  const M q = r * (r * (c.inv_n * cueq::warp_sum(dot))) * step;
+  CUEQ_CHANNELS {
+    const M a = cc[u], b = MODE == kBoth ? cw[u] * rh : M(0);
+    CUEQ_COMPONENTS {
+      M o = kPut || MODE == kBranch || has_go ? to<M>(go[CUEQ_AT]) : M(0);
+      if (MODE == kBoth && !kPut) o += b * to<M>(gn[CUEQ_AT]) - qh * to<M>(h[CUEQ_AT]);
+      const T dy = from<T>(a * o - q * to<M>(y[CUEQ_AT]));
+      if (MODE == kBoth && !kPut) go[CUEQ_AT] = from<T>(o);
+      (MODE == kBoth ? gn : go)[CUEQ_AT] = dy;
     }
-    if (c.gated && !Q8) dg[u] = from<T>(c.s[u] * dv * r * p);
   }
 }
 
-// ---- moving items -------------------------------------------------------------------------------------------------------
+// ---- one (row, irrep block) of at most 128 channels: a lane's K channels in registers ------------------------------------------------
+// Read from shared memory once, written once.  32 K is the number of channels or above it.
+template <class T, class M, int DIM, bool MUL_IR, int K>
+struct Short {
+  int lane, mul;
+  __device__ __forceinline__ bool ok(int k) const { return lane + 32 * k < mul; }
+  __device__ __forceinline__ int at(int k, int i) const { return MUL_IR ? (lane + 32 * k) * DIM + i : i * mul + lane + 32 * k; }
+  template <class E>
+  __device__ __forceinline__ void load(const E* p, M (&v)[K][DIM]) const {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < DIM; ++i) v[k][i] = ok(k) ? to<M>(p[at(k, i)]) : M(0);
+  }
+  __device__ __forceinline__ void store(T* p, const M (&v)[K][DIM]) const {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < DIM; ++i) if (ok(k)) p[at(k, i)] = from<T>(v[k][i]);
+  }
+  __device__ __forceinline__ void store_codes(signed char* p, const M (&v)[K][DIM], float inverse) const {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < DIM; ++i) if (ok(k)) p[at(k, i)] = to_code(v[k][i], inverse);
+  }
+  __device__ __forceinline__ M squares(const M (&v)[K][DIM]) const {
+    M part[DIM];
+#pragma unroll
+    for (int i = 0; i < DIM; ++i) part[i] = v[0][i] * v[0][i];
+#pragma unroll
+    for (int k = 1; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < DIM; ++i) part[i] += v[k][i] * v[k][i];
+#pragma unroll
+    for (int i = 1; i < DIM; ++i) part[0] += part[i];
+    return part[0];
+  }
+  __device__ __forceinline__ unsigned top(const M (&v)[K][DIM]) const {
+    unsigned t = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < DIM; ++i) t = max(t, magnitude(v[k][i]));
+    return __reduce_max_sync(0xffffffffu, t);
+  }
+};
+
+template <class T, class M, int MODE, bool Q8, int DIM, bool MUL_IR, int K>
+__device__ __forceinline__ void forward_short(const View<M>& c, T* x, T* y, const T* g, signed char* ca, signed char* cg, signed char* ch, M* stats) {
+  const Short<T, M, DIM, MUL_IR, K> q{c.lane, c.mul};
+  M v[K][DIM], a[K];
+  q.load((MODE & kBranch) ? y : x, v);
+  M xv[K][DIM];
+  if (MODE & kBranch) q.load(x, xv);
+#pragma unroll
+  for (int k = 0; k < K; ++k) a[k] = q.ok(k) ? ((MODE & kBranch) ? c.s : c.w)[c.lane + 32 * k] : M(0);
+  float gstep = 0.f, ginv = 0.f;
+  if ((MODE & kBranch) && c.gated) {
+    M gate[K];
+    unsigned gtop = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      gate[k] = q.ok(k) ? to<M>(g[c.lane + 32 * k]) : M(0);
+      if (Q8) gtop = max(gtop, magnitude(gate[k]));
+    }
+    if (Q8) code_step(__reduce_max_sync(0xffffffffu, gtop), gstep, ginv);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      M e, de;
+      activation(c.gate, gate[k], e, de);
+      a[k] *= e;
+      if (Q8 && q.ok(k)) cg[c.lane + 32 * k] = to_code(gate[k], ginv);
+    }
+  }
+  const M r = inverse_sqrt(cueq::warp_sum(q.squares(v)) * c.inv_n + c.eps);
+  float step = 0.f, inv = 0.f;
+  if (Q8) {
+    code_step(q.top(v), step, inv);
+    q.store_codes(ca, v, inv);
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < DIM; ++i) v[k][i] = (MODE & kBranch) ? xv[k][i] + a[k] * r * v[k][i] : a[k] * r * v[k][i];
+  q.store(x, v);
+  M rh = M(0);
+  float hstep = 0.f, hinv = 0.f;
+  if (MODE == kBoth) {
+    rh = inverse_sqrt(cueq::warp_sum(q.squares(v)) * c.inv_n + c.eps);
+    if (Q8) {
+      code_step(q.top(v), hstep, hinv);
+      q.store_codes(ch, v, hinv);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const M b = q.ok(k) ? c.w[c.lane + 32 * k] * rh : M(0);
+#pragma unroll
+      for (int i = 0; i < DIM; ++i) v[k][i] *= b;
+    }
+    q.store(y, v);
+  }
+  if (stats && c.lane == 0) {
+    stats[0] = r; stats[1] = rh; stats[2] = M(step); stats[3] = M(gstep);
+    if (Q8 && MODE == kBoth) stats[4] = M(hstep);
+  }
+}
+
+template <class T, class M, class K8, int MODE, bool Q8, int DIM, bool MUL_IR, int K>
+__device__ __forceinline__ void backward_short(const View<M>& c, T* go, T* gn, const K8* h, const K8* y, const K8* g, T* dg, const M* stats, bool has_go) {
+  const Short<T, M, DIM, MUL_IR, K> q{c.lane, c.mul};
+  M o[K][DIM], v[K][DIM];
+  if (MODE & kNorm) {
+    const M rh = stats[MODE == kBoth ? 1 : 0], step = Q8 ? stats[MODE == kBoth ? 4 : 2] : M(1);
+    q.load(gn, o);
+    q.load(h, v);
+    M dot = M(0), b[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      M p = M(0);
+#pragma unroll
+      for (int i = 0; i < DIM; ++i) p += o[k][i] * v[k][i];
+      p *= rh * step;
+      b[k] = q.ok(k) ? c.w[c.lane + 32 * k] : M(0);
+      if (q.ok(k)) c.acc_w[c.lane + 32 * k] += p;
+      dot += b[k] * p;
+    }
+    const M qh = rh * (rh * (c.inv_n * cueq::warp_sum(dot))) * step;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < DIM; ++i) o[k][i] = b[k] * rh * o[k][i] - qh * v[k][i];
+    if (MODE == kNorm) {
+      q.store(gn, o);
+      return;
+    }
+    if (has_go) {
+      q.load(go, v);
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < DIM; ++i) o[k][i] += v[k][i];
+    }
+    q.store(go, o);
+  } else {
+    q.load(go, o);
+  }
+  const M r = stats[0], step = Q8 ? stats[2] : M(1), gstep = Q8 ? stats[3] : M(1);
+  q.load(y, v);
+  M dot = M(0), a[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int u = c.lane + 32 * k;
+    M e = M(1), de = M(0), p = M(0);
+    if (c.gated) activation(c.gate, q.ok(k) ? to<M>(g[u]) * gstep : M(0), e, de);
+#pragma unroll
+    for (int i = 0; i < DIM; ++i) p += o[k][i] * v[k][i];
+    p *= r * step;
+    const M s = q.ok(k) ? c.s[u] : M(0);
+    a[k] = s * e;
+    dot += a[k] * p;
+    if (q.ok(k)) {
+      c.acc_s[u] += e * p;
+      if (c.gated) dg[u] = from<T>(s * de * p);          // may lie over g[u]
+    }
+  }
+  const M qy = r * (r * (c.inv_n * cueq::warp_sum(dot))) * step;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < DIM; ++i) v[k][i] = a[k] * r * o[k][i] - qy * v[k][i];
+  q.store(MODE == kBoth ? gn : go, v);
+}
+
+// ---- moving rows ----------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void bulk_in(void* dst, const void* src, unsigned bytes, unsigned long long* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
                ::"r"(s32(dst)), "l"(src), "r"(bytes), "r"(s32(bar)) : "memory");
@@ -351,182 +513,235 @@ __device__ __forceinline__ void bulk_in(void* dst, const void* src, unsigned byt
 __device__ __forceinline__ void bulk_out(void* dst, const void* src, unsigned bytes) {
   asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n" ::"l"(dst), "r"(s32(src)), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;\n" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory"); }
 
-// A region of a stage and the rows in memory that it holds: `size` bytes an element (1: codes).
-struct Move { int region, pitch, bytes, size; const unsigned char* src; unsigned char* dst; int64_t ld; };
+// A tensor's rows in memory and their region; elements of `size` bytes (codes and statistics: 16).  The last stage of a dense tensor may hold
+// bytes behind the last 16: these move like kPlain.
+struct Move { Region reg; int size, route; unsigned char* mem; int64_t ld; };
 
-// Rows [z0, z0 + n) of every region, plain: consecutive threads take consecutive elements.
-__device__ __forceinline__ void copy_rows(const Move& m, unsigned char* stage, int64_t z0, int n, bool in) {
-  for (int r = 0; r < n; ++r) {
-    unsigned char* a = stage + m.region + r * m.pitch;
-    if (in) {
-      const unsigned char* b = m.src + (z0 + r) * m.ld;
-      if (m.size == 2) for (int e = threadIdx.x; e < m.bytes / 2; e += kThreads) reinterpret_cast<unsigned short*>(a)[e] = __ldg(reinterpret_cast<const unsigned short*>(b) + e);
-      else if (m.size == 4) for (int e = threadIdx.x; e < m.bytes / 4; e += kThreads) reinterpret_cast<unsigned*>(a)[e] = __ldg(reinterpret_cast<const unsigned*>(b) + e);
-      else if (m.size == 8) for (int e = threadIdx.x; e < m.bytes / 8; e += kThreads) reinterpret_cast<unsigned long long*>(a)[e] = __ldg(reinterpret_cast<const unsigned long long*>(b) + e);
-      else for (int e = threadIdx.x; e < m.bytes / 16; e += kThreads) reinterpret_cast<uint4*>(a)[e] = __ldg(reinterpret_cast<const uint4*>(b) + e);
-    } else {
-      unsigned char* b = m.dst + (z0 + r) * m.ld;
-      if (m.size == 2) for (int e = threadIdx.x; e < m.bytes / 2; e += kThreads) reinterpret_cast<unsigned short*>(b)[e] = reinterpret_cast<unsigned short*>(a)[e];
-      else if (m.size == 4) for (int e = threadIdx.x; e < m.bytes / 4; e += kThreads) reinterpret_cast<unsigned*>(b)[e] = reinterpret_cast<unsigned*>(a)[e];
-      else if (m.size == 8) for (int e = threadIdx.x; e < m.bytes / 8; e += kThreads) reinterpret_cast<unsigned long long*>(b)[e] = reinterpret_cast<unsigned long long*>(a)[e];
-      else for (int e = threadIdx.x; e < m.bytes / 16; e += kThreads) reinterpret_cast<uint4*>(b)[e] = reinterpret_cast<uint4*>(a)[e];
-    }
+template <bool IN, class E>
+__device__ __forceinline__ void copy_elements(unsigned char* smem, unsigned char* mem, int from, int bytes, int lane) {
+  E *a = reinterpret_cast<E*>(smem), *b = reinterpret_cast<E*>(mem);
+  for (int e = from / (int)sizeof(E) + lane; e < bytes / (int)sizeof(E); e += 32) {
+    if (IN) a[e] = __ldg(b + e); else b[e] = a[e];
+  }
+}
+template <bool IN>
+__device__ __forceinline__ void copy_row(unsigned char* smem, unsigned char* mem, int from, int bytes, int size, int lane) {
+  switch (size) {
+    case 2: copy_elements<IN, unsigned short>(smem, mem, from, bytes, lane); break;
+    case 4: copy_elements<IN, unsigned>(smem, mem, from, bytes, lane); break;
+    case 8: copy_elements<IN, unsigned long long>(smem, mem, from, bytes, lane); break;
+    default: copy_elements<IN, uint4>(smem, mem, from, bytes, lane); break;
+  }
+}
+template <bool IN>
+__device__ __noinline__ void copy_rest(const Move* moves, int count, unsigned char* stage, int64_t z, int n) {
+  const int lane = threadIdx.x;
+  for (int k = 0; k < count; ++k) {
+    const Move& m = moves[k];
+    unsigned char *a = stage + m.reg.at, *b = m.mem + z * m.ld;
+    if (m.route == kPlain) for (int r = 0; r < n; ++r) copy_row<IN>(a + r * m.reg.pitch, b + r * m.ld, 0, m.reg.bytes, m.size, lane);
+    if (m.route == kDense) copy_row<IN>(a, b, n * m.reg.bytes & ~15, n * m.reg.bytes, m.size, lane);
   }
 }
 
-// Rows first .. last in stages of rps rows: loads, work on a stage, stores.  Loads and stores of row r of a stage are issued by
-// lane r of warp 0, so that a lane's own wait for its stores' reads covers the memory that its next loads overwrite.
-template <int NIN, int NOUT, class Work>
-__device__ __forceinline__ void run_stages(const Params& p, const Blk& b, int64_t first, int64_t last, const Move (&in)[NIN], int nin,
-                                           const Move (&out)[NOUT], int nout, unsigned char* stages, int stage_bytes, unsigned long long* full,
-                                           Work work) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (!p.bulk) {
-    for (int64_t z = first; z < last; z += b.rps) {
-      const int n = (int)min((int64_t)b.rps, last - z);
-#pragma unroll
-      for (int k = 0; k < NIN; ++k) if (k < nin) copy_rows(in[k], stages, z, n, true);
-      __syncthreads();
-      work(stages, z, n);
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < NOUT; ++k) if (k < nout) copy_rows(out[k], stages, z, n, false);
-      __syncthreads();
+// The bulk copy that a lane issues per stage: one row of one tensor, or all rows of a dense one.
+static_assert(sizeof(Move) == kMoveBytes, "moves have their room in front of the stages");
+struct Job {
+  unsigned at;                       // inside a stage
+  int bytes, row;                    // of a row; a dense tensor: row = -1
+  unsigned char* mem;                // in the next stage
+  int64_t step;                      // from stage to stage
+  bool rest;                         // some tensor needs copy_rest
+};
+__device__ __forceinline__ Job make_job(const Move* moves, int count, int rps, int64_t first) {
+  Job j{0u, 0, 0, nullptr, 0, false};
+  int at = 0;
+  for (int k = 0; k < count; ++k) {
+    const Move& m = moves[k];
+    if (m.route == kPlain) { j.rest = true; continue; }
+    const int lanes = m.route == kDense ? 1 : rps, r = (int)threadIdx.x - at;
+    if (r >= 0 && r < lanes) {
+      j.at = m.reg.at + r * m.reg.pitch;
+      j.bytes = m.reg.bytes;
+      j.row = m.route == kDense ? -1 : r;
+      j.mem = m.mem + (first + r) * m.ld;
+      j.step = rps * m.ld;
     }
-    return;
+    at += lanes;
   }
-  unsigned row_bytes = 0;
-#pragma unroll
-  for (int k = 0; k < NIN; ++k) if (k < nin) row_bytes += in[k].bytes;
+  return j;
+}
+// bytes that this lane's copy has with n rows in the stage
+__device__ __forceinline__ unsigned job_bytes(const Job& j, int n) { return j.row < 0 ? (unsigned)(n * j.bytes) & ~15u : j.row < n ? j.bytes : 0u; }
+
+// Rows first .. last in stages of rps rows; `work(stage, z, n)`.  A lane that issues loads into a stage waits for its own stores out of
+// it; the warp then meets, so that no lane's load overtakes another lane's store.  One stage at a time where two do not fit.
+template <class Work>
+__device__ __forceinline__ void run_stages(const Params& p, int rps, int64_t first, int64_t last, const Move* in, int nin, const Move* out, int nout,
+                                           unsigned char* stages, int stage_bytes, unsigned long long* full, Work work) {
+  const int lane = threadIdx.x;
+  Job jin = make_job(in, nin, rps, first), jout = make_job(out, nout, rps, first);
   auto load = [&](int64_t z, int s) {
-    const int n = (int)min((int64_t)b.rps, last - z);
-    if (lane == 0) bar_expect_tx(full + s, n * row_bytes);
+    const int n = (int)min((int64_t)rps, last - z);
+    unsigned char* stage = stages + s * stage_bytes;
+    const unsigned bytes = job_bytes(jin, n), sum = __reduce_add_sync(0xffffffffu, bytes);
+    if (lane == 0) bar_expect_tx(full + s, sum);         // none: the arrival alone completes the phase
     __syncwarp();
-    if (lane < n) {
-#pragma unroll
-      for (int k = 0; k < NIN; ++k)
-        if (k < nin) bulk_in(stages + s * stage_bytes + in[k].region + lane * in[k].pitch, in[k].src + (z + lane) * in[k].ld, in[k].bytes, full + s);
-    }
+    if (bytes) bulk_in(stage + jin.at, jin.mem, bytes, full + s);
+    jin.mem += jin.step;
+    if (jin.rest || n < rps) copy_rest<true>(in, nin, stage, z, n);
   };
-  if (warp == 0 && first < last) load(first, 0);
-  unsigned it = 0;
-  for (int64_t z = first; z < last; z += b.rps, ++it) {
-    const int s = it & 1, n = (int)min((int64_t)b.rps, last - z);
-    const bool more = z + b.rps < last;
-    if (warp == 0 && more) {
-      bulk_wait_read();                                  // this lane's stores from the other stage
-      load(z + b.rps, s ^ 1);
+  const bool two = p.stages == 2;
+  if (first < last) load(first, 0);
+  int s = 0;
+  unsigned phases = 0;                                   // bit s: the phase that stage s waits for
+  for (int64_t z = first; z < last; z += rps) {
+    const int n = (int)min((int64_t)rps, last - z);
+    const bool more = z + rps < last;
+    if (two && more) {
+      asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
+      __syncwarp();
+      load(z + rps, s ^ 1);
     }
-    const bool ok = bar_wait(full + s, (it >> 1) & 1, p.status);
-    if (!__syncthreads_and(ok)) {                        // a copy did not arrive in time: give up once the copies in flight have landed
-      if (more) bar_wait(full + (s ^ 1), ((it + 1) >> 1) & 1, p.status);
-      bar_wait(full + s, (it >> 1) & 1, p.status);
+    if (!__all_sync(0xffffffffu, bar_wait(full + s, phases >> s & 1, p.status))) {   // a copy did not arrive in time: give up once those in flight have landed
+      if (two && more) bar_wait(full + (s ^ 1), phases >> (s ^ 1) & 1, p.status);
+      bar_wait(full + s, phases >> s & 1, p.status);
       break;
     }
-    work(stages + s * stage_bytes, z, n);
+    phases ^= 1u << s;
+    unsigned char* stage = stages + s * stage_bytes;
+    work(stage, z, n);
     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-    __syncthreads();
-    if (warp == 0) {
-      if (lane < n) {
-#pragma unroll
-        for (int k = 0; k < NOUT; ++k)
-          if (k < nout) bulk_out(out[k].dst + (z + lane) * out[k].ld, stages + s * stage_bytes + out[k].region + lane * out[k].pitch, out[k].bytes);
-      }
-      bulk_commit();
+    __syncwarp();
+    const unsigned bytes = job_bytes(jout, n);
+    if (bytes) bulk_out(jout.mem, stage + jout.at, bytes);
+    asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+    jout.mem += jout.step;
+    if (jout.rest || n < rps) copy_rest<false>(out, nout, stage, z, n);
+    if (two) s ^= 1;
+    else if (more) {
+      asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
+      __syncwarp();
+      load(z + rps, 0);
     }
   }
-  if (warp == 0) bulk_wait_read();
+  asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
 }
 
+__device__ __forceinline__ const Slice& my_slice(const Params& p) {
+  int k = 0;
+  while (k + 1 < p.num_slices && (int)blockIdx.x >= p.slice[k + 1].cta0) ++k;
+  return p.slice[k];
+}
+// parameters of the slice's channels into shared memory, sums cleared, barriers
 template <class M>
-__device__ __forceinline__ View<M> make_view(const Params& p, const Blk& b, unsigned char* smem, bool backward) {
-  View<M> c;
-  c.mul = b.mul; c.dim = b.dim; c.n = b.mul * b.dim;
-  c.su = p.mul_ir ? b.dim : 1;
-  c.si = p.mul_ir ? 1 : b.mul;
-  c.wpi = b.wpi;
-  const int warp = threadIdx.x >> 5;
-  c.lane = threadIdx.x & 31;
-  c.group = warp / b.wpi;
-  c.warp_in = warp % b.wpi;
-  c.tg = c.warp_in * 32 + c.lane;
-  c.gt = b.wpi * 32;
-  c.gate = p.gate; c.gated = p.gate != CUEQ_NORM_GATE_NONE;
-  c.inv_n = M(1) / M(c.n);
-  c.eps = M(p.eps);
-  c.red = smem + kRed;
-  c.red_at = 0;
-  c.s = reinterpret_cast<M*>(smem + kRed + kRedBytes);
-  c.w = c.s + b.mul;
-  c.acc_s = c.w + b.mul + c.group * b.mul;
-  c.acc_w = c.w + b.mul + (kWarps / b.wpi + c.group) * b.mul;
-  for (int u = threadIdx.x; u < b.mul; u += kThreads) {
-    c.s[u] = p.s ? cueq::load_as<M>(p.s, p.pdtype, b.ch + u) : M(1);
-    c.w[u] = p.w ? cueq::load_as<M>(p.w, p.pdtype, b.ch + u) : M(1);
+__device__ __forceinline__ M* prepare(const Params& p, const Slice& s, unsigned char* smem, bool backward) {
+  M* at = reinterpret_cast<M*>(smem + kBars);
+  const int ch = p.blk[s.first].ch, n = s.channels;
+  for (int u = threadIdx.x; u < n; u += 32) {
+    at[u] = p.s ? cueq::load_as<M>(p.s, p.pdtype, ch + u) : M(1);
+    at[n + u] = p.w ? cueq::load_as<M>(p.w, p.pdtype, ch + u) : M(1);
+    if (backward) at[3 * n + u] = at[4 * n + u] = M(0);
   }
-  if (backward)
-    for (int u = threadIdx.x; u < 2 * (kWarps / b.wpi) * b.mul; u += kThreads) c.w[b.mul + u] = M(0);
   if (threadIdx.x == 0) {
     bar_init(reinterpret_cast<unsigned long long*>(smem), 1);
     bar_init(reinterpret_cast<unsigned long long*>(smem) + 1, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  __syncthreads();
+  __syncwarp();
+  return at;
+}
+template <class M>
+__device__ __forceinline__ View<M> block_view(const Params& p, const Slice& s, const Blk& b, M* at) {
+  View<M> c;
+  const int u0 = b.ch - p.blk[s.first].ch, n = s.channels;
+  c.s = at + u0; c.w = at + n + u0; c.a = at + 2 * n + u0; c.acc_s = at + 3 * n + u0; c.acc_w = at + 4 * n + u0;
+  c.mul = b.mul; c.dim = b.dim;
+  c.lane = threadIdx.x;
+  c.gate = p.gate; c.gated = p.gate != CUEQ_NORM_GATE_NONE;
+  c.inv_n = M(b.inv_n);
+  c.eps = M(p.eps);
   return c;
 }
 
-__device__ __forceinline__ const Blk& my_block(const Params& p) {
-  int k = 0;
-  while (k + 1 < p.nb && (int)blockIdx.x >= p.blk[k + 1].cta0) ++k;
-  return p.blk[k];
+template <int NIN, int NOUT>
+__device__ __forceinline__ void put_moves(Move* moves, const Move (&in)[NIN], int nin, const Move (&out)[NOUT], int nout) {
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int k = 0; k < NIN; ++k) if (k < nin) moves[k] = in[k];
+#pragma unroll
+    for (int k = 0; k < NOUT; ++k) if (k < nout) moves[nin + k] = out[k];
+  }
+  __syncwarp();
 }
 
-#define CUEQ_NORM_DIMS(dim, CALL)      \
-  switch (dim) {                       \
-    case 1: { CALL(1); break; }        \
-    case 3: { CALL(3); break; }        \
-    case 5: { CALL(5); break; }        \
-    case 7: { CALL(7); break; }        \
-    default: { CALL(0); break; }       \
+// (dimension, channels per lane) of a block: CALL for those that registers hold, LONG for the others
+#define CUEQ_NORM_K(D, CALL) if (b.mul <= 32) CALL(D, 1); else if (b.mul <= 64) CALL(D, 2); else CALL(D, 4)
+#define CUEQ_NORM_DIMS(CALL, LONG)                                                     \
+  if (b.mul <= 128 && b.dim <= 7) {                                                    \
+    switch (b.dim) {                                                                   \
+      case 1: CUEQ_NORM_K(1, CALL); break;                                             \
+      case 3: CUEQ_NORM_K(3, CALL); break;                                             \
+      case 5: CUEQ_NORM_K(5, CALL); break;                                             \
+      default: CUEQ_NORM_K(7, CALL); break;                                            \
+    }                                                                                  \
+  } else {                                                                             \
+    switch (b.dim) {                                                                   \
+      case 1: LONG(1); break;                                                          \
+      case 3: LONG(3); break;                                                          \
+      case 5: LONG(5); break;                                                          \
+      case 7: LONG(7); break;                                                          \
+      default: LONG(0); break;                                                         \
+    }                                                                                  \
   }
 
-template <class T, class M, int MODE, bool Q8>
-__global__ void __launch_bounds__(kThreads, sizeof(M) == 8 ? 4 : 8) forward_kernel(const __grid_constant__ Params p) {
+template <class T, class M, int MODE, bool Q8, bool MUL_IR>
+__global__ void __launch_bounds__(32, warps_per_sm(sizeof(M))) forward_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) unsigned char smem[];
-  const Blk& b = my_block(p);
-  View<M> c = make_view<M>(p, b, smem, false);
-  const int j = blockIdx.x - b.cta0, size = sizeof(T);
-  const int64_t first = p.rows * j / b.ncta, last = p.rows * (j + 1) / b.ncta;
-  const Stage st = forward_stage(MODE, Q8, c.gated, size, b.mul, b.dim, b.rps);
-  const int item = b.mul * b.dim * size, gate = b.mul * size, code = pad16(b.mul * b.dim), gcode = pad16(b.mul);
-  const bool branch = MODE & kBranch;
-  auto at = [](const void* q, int64_t bytes) { return reinterpret_cast<unsigned char*>(const_cast<void*>(q)) + bytes; };
-  const int64_t ldo = (int64_t)p.dim_total * size;
-  const Move in[3] = {{st.a, pad16(item), item, size, at(p.x, (int64_t)b.off * size), nullptr, p.ldx * size},
-                      {st.b, pad16(item), item, size, at(p.y, (int64_t)b.off * size), nullptr, p.ldy * size},
-                      {st.g, pad16(gate), gate, size, at(p.g, (int64_t)b.ch * size), nullptr, p.ldg * size}};
-  const Move o_out = {st.a, pad16(item), item, size, nullptr, at(branch ? p.out : p.norm, (int64_t)b.off * size), ldo};
-  const Move o_norm = {st.b, pad16(item), item, size, nullptr, at(p.norm, (int64_t)b.off * size), ldo};
-  const Move o_ca = {st.ca, code, code, 16, nullptr, (unsigned char*)p.codes + b.code, p.ldc};
-  const Move o_cg = {st.cg, gcode, gcode, 16, nullptr, (unsigned char*)p.codes + b.gcode, p.ldc};
-  const Move o_cb = {st.cb, code, code, 16, nullptr, (unsigned char*)p.codes + b.hcode, p.ldc};
-  // results in an order in which those that a call does not have come last
-  const Move out[5] = {o_out, MODE == kBoth ? o_norm : o_ca, MODE == kBoth ? o_ca : o_cg, MODE == kBoth ? o_cb : o_cg, o_cg};
-  const int nout = 1 + (MODE == kBoth) + (Q8 ? 1 + (MODE == kBoth) + (branch && c.gated) : 0);
-  const int k = (int)(&b - p.blk);
-  run_stages(p, b, first, last, in, branch ? 2 + c.gated : 1, out, nout, smem + head_bytes(sizeof(M), b.mul, false, b.wpi), st.total,
+  const Slice& sl = my_slice(p);
+  M* at = prepare<M>(p, sl, smem, false);
+  constexpr int size = sizeof(T);
+  const int64_t units = (p.rows + sl.rps - 1) / sl.rps, j = blockIdx.x - sl.cta0;
+  const int64_t first = units * j / sl.ncta * sl.rps, last = min(p.rows, units * (j + 1) / sl.ncta * sl.rps);
+  const Stage st = forward_stage(p, sl, MODE, Q8, size);
+  const Blk& b0 = p.blk[sl.first];
+  const bool gated = (MODE & kBranch) && p.gate != CUEQ_NORM_GATE_NONE;
+  auto ptr = [](const void* q, int64_t bytes) { return reinterpret_cast<unsigned char*>(const_cast<void*>(q)) + bytes; };
+  const int64_t fo = (int64_t)b0.off * size, ldo = (int64_t)p.dim_total * size;
+  Move* moves = reinterpret_cast<Move*>(smem + 16);
+  const Move in[3] = {{st.a, size, p.route[tX], ptr(p.x, fo), p.ldx * size},
+                      {st.b, size, p.route[tY], ptr(p.y, fo), p.ldy * size},
+                      {st.g, size, p.route[tG], ptr(p.g, (int64_t)b0.ch * size), p.ldg * size}};
+  const Move o_first = {st.a, size, p.route[(MODE & kBranch) ? tOut : tNorm], ptr((MODE & kBranch) ? p.out : p.norm, fo), ldo};
+  const Move o_norm = {st.b, size, p.route[tNorm], ptr(p.norm, fo), ldo};
+  const Move o_ca = {st.ca, 16, kRows, (unsigned char*)p.codes + b0.code, p.ldc};
+  const Move o_cg = {st.cg, 16, kRows, (unsigned char*)p.codes + b0.gcode, p.ldc};
+  const Move o_ch = {st.ch, 16, kRows, (unsigned char*)p.codes + b0.hcode, p.ldc};
+  // those that a call does not have come last
+  const Move out[5] = {o_first, MODE == kBoth ? o_norm : o_ca, MODE == kBoth ? o_ca : o_cg, MODE == kBoth ? o_ch : o_cg, o_cg};
+  const int nout = 1 + (MODE == kBoth) + (Q8 ? 1 + (MODE == kBoth) + gated : 0);
+  const int nin = (MODE & kBranch) ? 2 + gated : 1;
+  put_moves(moves, in, nin, out, nout);
+  run_stages(p, sl.rps, first, last, moves, nin, moves + nin, nout, smem + head_bytes(sizeof(M), sl.channels, false), st.total,
              reinterpret_cast<unsigned long long*>(smem), [&](unsigned char* s, int64_t z, int n) {
-    for (int r = c.group; r < n; r += kWarps / c.wpi) {
-      M* stats = p.stats ? reinterpret_cast<M*>(p.stats) + ((z + r) * p.nb + k) * p.ns : nullptr;
-#define CUEQ_CALL(D)                                                                                                              \
-  forward_item<T, M, MODE, Q8, D>(c, reinterpret_cast<T*>(s + st.a + r * pad16(item)), reinterpret_cast<T*>(s + st.b + r * pad16(item)), \
-                                  reinterpret_cast<const T*>(s + st.g + r * pad16(gate)), reinterpret_cast<signed char*>(s + st.ca + r * code), \
-                                  reinterpret_cast<signed char*>(s + st.cg + r * gcode), reinterpret_cast<signed char*>(s + st.cb + r * code), stats)
-      CUEQ_NORM_DIMS(b.dim, CUEQ_CALL)
+    for (int k = sl.first; k < sl.first + sl.count; ++k) {
+      const Blk& b = p.blk[k];
+      const View<M> c = block_view<M>(p, sl, b, at);
+      const int e = b.off - b0.off, u = b.ch - b0.ch;
+      for (int r = 0; r < n; ++r) {
+        M* stats = p.stats ? reinterpret_cast<M*>(p.stats) + ((z + r) * p.nb + k) * p.ns : nullptr;
+        T *px = reinterpret_cast<T*>(s + st.a.at + r * st.a.pitch) + e, *py = reinterpret_cast<T*>(s + st.b.at + r * st.b.pitch) + e;
+        const T* pg = reinterpret_cast<const T*>(s + st.g.at + r * st.g.pitch) + u;
+        signed char *pa = reinterpret_cast<signed char*>(s + st.ca.at + r * st.ca.pitch) + (b.code - b0.code),
+                    *pc = reinterpret_cast<signed char*>(s + st.cg.at + r * st.cg.pitch) + (b.gcode - b0.gcode),
+                    *ph = reinterpret_cast<signed char*>(s + st.ch.at + r * st.ch.pitch) + (b.hcode - b0.hcode);
+#define CUEQ_CALL(D, K) forward_short<T, M, MODE, Q8, D, MUL_IR, K>(c, px, py, pg, pa, pc, ph, stats)
+#define CUEQ_LONG(D) forward_item<T, M, MODE, Q8, D, MUL_IR>(c, px, py, pg, pa, pc, ph, stats)
+        CUEQ_NORM_DIMS(CUEQ_CALL, CUEQ_LONG)
+#undef CUEQ_LONG
 #undef CUEQ_CALL
+      }
     }
   });
 }
@@ -534,75 +749,87 @@ __global__ void __launch_bounds__(kThreads, sizeof(M) == 8 ? 4 : 8) forward_kern
 template <class T, bool Q8> struct Kept { using type = T; };
 template <class T> struct Kept<T, true> { using type = signed char; };
 
-template <class T, class M, int MODE, bool Q8>
-__global__ void __launch_bounds__(kThreads, sizeof(M) == 8 ? 4 : 8) backward_kernel(const __grid_constant__ Params p) {
+template <class T, class M, int MODE, bool Q8, bool MUL_IR>
+__global__ void __launch_bounds__(32, warps_per_sm(sizeof(M))) backward_kernel(const __grid_constant__ Params p) {
   using K = typename Kept<T, Q8>::type;
   extern __shared__ __align__(128) unsigned char smem[];
-  const Blk& b = my_block(p);
-  View<M> c = make_view<M>(p, b, smem, true);
-  const int j = blockIdx.x - b.cta0, size = sizeof(T);
-  const int64_t first = p.rows * j / b.ncta, last = p.rows * (j + 1) / b.ncta;
+  const Slice& sl = my_slice(p);
+  M* at = prepare<M>(p, sl, smem, true);
+  constexpr int size = sizeof(T);
   const int stat = p.ns * (int)sizeof(M);
-  const Stage st = backward_stage(MODE, Q8, c.gated, size, b.mul, b.dim, b.rps, stat);
-  const int item = b.mul * b.dim * size, gate = b.mul * size, code = pad16(b.mul * b.dim), gcode = pad16(b.mul);
-  const bool branch = MODE & kBranch, has_go = p.go != nullptr;
-  auto at = [](const void* q, int64_t bytes) { return reinterpret_cast<unsigned char*>(const_cast<void*>(q)) + bytes; };
-  const int64_t fo = (int64_t)b.off * size, go_ = (int64_t)b.ch * size, ldo = (int64_t)p.dim_total * size;
-  const int kpitch = Q8 ? code : pad16(item), kbytes = Q8 ? code : item, ksize = Q8 ? 16 : size;
-  const int k = (int)(&b - p.blk);
-  const Move i_go = {st.a, pad16(item), item, size, at(p.go, fo), nullptr, p.ldgo * size};
-  const Move i_gn = {st.b, pad16(item), item, size, at(p.gn, fo), nullptr, p.ldgn * size};
-  const Move i_h = {st.c, kpitch, kbytes, ksize, Q8 ? (unsigned char*)p.codes + (MODE == kBoth ? b.hcode : b.code) : at(p.h, fo), nullptr,
-                    Q8 ? p.ldc : p.ldh * size};
-  const Move i_y = {st.d, kpitch, kbytes, ksize, Q8 ? (unsigned char*)p.codes + b.code : at(p.y, fo), nullptr, Q8 ? p.ldc : p.ldy * size};
-  const Move i_g = {st.g, Q8 ? gcode : pad16(gate), Q8 ? gcode : gate, Q8 ? 16 : size, Q8 ? (unsigned char*)p.codes + b.gcode : at(p.g, go_),
-                    nullptr, Q8 ? p.ldc : p.ldg * size};
-  const Move i_st = {st.st, stat, stat, 16, (unsigned char*)p.stats + (int64_t)k * stat, nullptr, (int64_t)p.nb * stat};
-  // operands in an order in which those that a call does not have come last
+  const int64_t units = (p.rows + sl.rps - 1) / sl.rps, j = blockIdx.x - sl.cta0;
+  const int64_t first = units * j / sl.ncta * sl.rps, last = min(p.rows, units * (j + 1) / sl.ncta * sl.rps);
+  const Stage st = backward_stage(p, sl, MODE, Q8, size, stat);
+  const Blk& b0 = p.blk[sl.first];
+  const bool branch = MODE & kBranch, gated = branch && p.gate != CUEQ_NORM_GATE_NONE, has_go = p.go != nullptr;
+  auto ptr = [](const void* q, int64_t bytes) { return reinterpret_cast<unsigned char*>(const_cast<void*>(q)) + bytes; };
+  const int64_t fo = (int64_t)b0.off * size, uo = (int64_t)b0.ch * size, ldo = (int64_t)p.dim_total * size;
+  unsigned char* codes = (unsigned char*)p.codes;
+  Move* moves = reinterpret_cast<Move*>(smem + 16);
+  const Move i_st = {st.st, 16, p.route[tStats], (unsigned char*)p.stats + (int64_t)sl.first * stat, (int64_t)p.nb * stat};
+  const Move i_go = {st.a, size, p.route[tGo], ptr(p.go, fo), p.ldgo * size};
+  const Move i_gn = {st.b, size, p.route[tGn], ptr(p.gn, fo), p.ldgn * size};
+  const Move i_h = Q8 ? Move{st.c, 16, kRows, codes + (MODE == kBoth ? b0.hcode : b0.code), p.ldc} : Move{st.c, size, p.route[tH], ptr(p.h, fo), p.ldh * size};
+  const Move i_y = Q8 ? Move{st.d, 16, kRows, codes + b0.code, p.ldc} : Move{st.d, size, p.route[tY], ptr(p.y, fo), p.ldy * size};
+  const Move i_g = Q8 ? Move{st.g, 16, kRows, codes + b0.gcode, p.ldc} : Move{st.g, size, p.route[tG], ptr(p.g, uo), p.ldg * size};
+  // those that a call does not have come last
   const Move in[6] = {i_st, branch ? i_y : i_h, branch ? (MODE == kBoth ? i_h : i_go) : i_gn, MODE == kBoth ? i_gn : i_g,
-                      MODE == kBoth && c.gated ? i_g : i_go, i_go};
-  const int nin = MODE == kNorm ? 3 : MODE == kBranch ? 3 + c.gated : 4 + c.gated + has_go;
-  const Move o_a = {st.a, pad16(item), item, size, nullptr, at(branch && MODE == kBoth ? p.dx : p.dy, fo), ldo};
-  const Move o_b = {st.b, pad16(item), item, size, nullptr, at(branch ? p.dy : p.dx, fo), ldo};
-  const Move o_g = {st.dg, pad16(gate), gate, size, nullptr, at(p.dg, go_), (int64_t)p.channels * size};
+                      MODE == kBoth && gated ? i_g : i_go, i_go};
+  const int nin = MODE == kNorm ? 3 : MODE == kBranch ? 3 + gated : 4 + gated + has_go;
+  const Move o_a = {st.a, size, p.route[MODE == kBoth ? tDx : tDy], ptr(MODE == kBoth ? p.dx : p.dy, fo), ldo};
+  const Move o_b = {st.b, size, p.route[branch ? tDy : tDx], ptr(branch ? p.dy : p.dx, fo), ldo};
+  const Move o_g = {st.dg, size, p.route[tDg], ptr(p.dg, uo), (int64_t)p.channels * size};
   const Move out[3] = {MODE == kNorm ? o_b : o_a, MODE == kBoth ? o_b : o_g, o_g};
-  const int nout = MODE == kNorm ? 1 : 1 + (MODE == kBoth) + c.gated;
-  run_stages(p, b, first, last, in, nin, out, nout, smem + head_bytes(sizeof(M), b.mul, true, b.wpi), st.total,
+  const int nout = MODE == kNorm ? 1 : 1 + (MODE == kBoth) + gated;
+  put_moves(moves, in, nin, out, nout);
+  run_stages(p, sl.rps, first, last, moves, nin, moves + nin, nout, smem + head_bytes(sizeof(M), sl.channels, true), st.total,
              reinterpret_cast<unsigned long long*>(smem), [&](unsigned char* s, int64_t, int n) {
-    for (int r = c.group; r < n; r += kWarps / c.wpi) {
-#define CUEQ_CALL(D)                                                                                                              \
-  backward_item<T, M, K, MODE, Q8, D>(c, reinterpret_cast<T*>(s + st.a + r * pad16(item)), reinterpret_cast<T*>(s + st.b + r * pad16(item)), \
-                                      reinterpret_cast<const K*>(s + st.c + r * kpitch), reinterpret_cast<const K*>(s + st.d + r * kpitch),  \
-                                      reinterpret_cast<const K*>(s + st.g + r * (Q8 ? gcode : pad16(gate))),                      \
-                                      reinterpret_cast<T*>(s + st.dg + r * pad16(gate)), reinterpret_cast<const M*>(s + st.st + r * stat), has_go)
-      CUEQ_NORM_DIMS(b.dim, CUEQ_CALL)
+    for (int k = sl.first; k < sl.first + sl.count; ++k) {
+      const Blk& b = p.blk[k];
+      const View<M> c = block_view<M>(p, sl, b, at);
+      const int e = b.off - b0.off, u = b.ch - b0.ch;
+      const int ce = Q8 ? b.code - b0.code : e, he = Q8 ? (MODE == kBoth ? b.hcode - b0.hcode : b.code - b0.code) : e, ge = Q8 ? b.gcode - b0.gcode : u;
+      for (int r = 0; r < n; ++r) {
+        T *pa = reinterpret_cast<T*>(s + st.a.at + r * st.a.pitch) + e, *pb = reinterpret_cast<T*>(s + st.b.at + r * st.b.pitch) + e;
+        const K *ph = reinterpret_cast<const K*>(s + st.c.at + r * st.c.pitch) + he, *py = reinterpret_cast<const K*>(s + st.d.at + r * st.d.pitch) + ce,
+                *pg = reinterpret_cast<const K*>(s + st.g.at + r * st.g.pitch) + ge;
+        T* pd = reinterpret_cast<T*>(s + st.dg.at + r * st.dg.pitch) + u;
+        const M* ps = reinterpret_cast<const M*>(s + st.st.at + r * st.st.pitch) + (k - sl.first) * p.ns;
+#define CUEQ_CALL(D, N) backward_short<T, M, K, MODE, Q8, D, MUL_IR, N>(c, pa, pb, ph, py, pg, pd, ps, has_go)
+#define CUEQ_LONG(D) backward_item<T, M, K, MODE, Q8, D, MUL_IR>(c, pa, pb, ph, py, pg, pd, ps, has_go)
+        CUEQ_NORM_DIMS(CUEQ_CALL, CUEQ_LONG)
+#undef CUEQ_LONG
 #undef CUEQ_CALL
+      }
     }
   });
-  // this thread block's sums of the parameters' gradients, its groups in order
-  __syncthreads();
-  const int ng = kWarps / b.wpi;
-  for (int u = threadIdx.x; u < b.mul; u += kThreads) {
-    M vs = M(0), vw = M(0);
-    for (int k2 = 0; k2 < ng; ++k2) { vs += c.w[b.mul + k2 * b.mul + u]; vw += c.w[b.mul + (ng + k2) * b.mul + u]; }
-    M* dst = reinterpret_cast<M*>(p.parts) + b.part + (int64_t)j * b.mul + u;
-    if (MODE & kBranch) dst[0] = vs;
-    if (MODE & kNorm) dst[p.parts_len] = vw;
+  // this warp's sums of the parameters' gradients
+  M* dst = reinterpret_cast<M*>(p.parts) + sl.part + j * sl.channels;
+  for (int u = threadIdx.x; u < sl.channels; u += 32) {
+    if (MODE & kBranch) dst[u] = at[3 * sl.channels + u];
+    if (MODE & kNorm) dst[p.parts_len + u] = at[4 * sl.channels + u];
   }
 }
 
 using Kernel = void (*)(Params);
 
-// the kernels of one element type, [mode - 1][q8]
-template <class T, class M, bool Q8>
+// the kernels of one element type
+template <class T, class M, bool Q8, bool MUL_IR>
 Kernel pick(int mode, bool backward) {
   if (backward)
-    return mode == kBranch ? backward_kernel<T, M, kBranch, Q8> : mode == kNorm ? backward_kernel<T, M, kNorm, Q8> : backward_kernel<T, M, kBoth, Q8>;
-  return mode == kBranch ? forward_kernel<T, M, kBranch, Q8> : mode == kNorm ? forward_kernel<T, M, kNorm, Q8> : forward_kernel<T, M, kBoth, Q8>;
+    return mode == kBranch ? backward_kernel<T, M, kBranch, Q8, MUL_IR> : mode == kNorm ? backward_kernel<T, M, kNorm, Q8, MUL_IR> : backward_kernel<T, M, kBoth, Q8, MUL_IR>;
+  return mode == kBranch ? forward_kernel<T, M, kBranch, Q8, MUL_IR> : mode == kNorm ? forward_kernel<T, M, kNorm, Q8, MUL_IR> : forward_kernel<T, M, kBoth, Q8, MUL_IR>;
 }
-Kernel pick_f32(int mode, bool q8, bool backward);
-Kernel pick_f64(int mode, bool q8, bool backward);
-Kernel pick_bf16(int mode, bool q8, bool backward);
-Kernel pick_f16(int mode, bool q8, bool backward);
+template <class T, class M>
+Kernel pick(int mode, bool q8, bool mul_ir, bool backward) {
+  if constexpr (sizeof(M) == 4) {
+    if (q8) return mul_ir ? pick<T, M, true, true>(mode, backward) : pick<T, M, true, false>(mode, backward);
+  }
+  return mul_ir ? pick<T, M, false, true>(mode, backward) : pick<T, M, false, false>(mode, backward);
+}
+Kernel pick_f32(int mode, bool q8, bool mul_ir, bool backward);
+Kernel pick_f64(int mode, bool q8, bool mul_ir, bool backward);
+Kernel pick_bf16(int mode, bool q8, bool mul_ir, bool backward);
+Kernel pick_f16(int mode, bool q8, bool mul_ir, bool backward);
 
 }  // namespace cueq_norm
