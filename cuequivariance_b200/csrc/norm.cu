@@ -10,7 +10,6 @@ using namespace cueq_norm;
 
 constexpr int kSmemPerSm = 227 * 1024, kSms = 148;
 constexpr int kSliceValues = 1024;       // neighbouring irrep blocks are put together up to this length
-constexpr int kItemCost = 64;            // what a (row, block) costs besides its values, in values
 constexpr int kStageBytes = 4096;        // rows are put together up to about this much per stage
 
 int element_size(int dtype) { return dtype == CUEQ_F64 ? 8 : dtype == CUEQ_F32 ? 4 : 2; }
@@ -92,13 +91,12 @@ int copy_lanes(const cueq_norm_args* a, bool backward, const Params& p, int rps)
   return in > out ? in : out;
 }
 
-// Divides the work: neighbouring irrep blocks to slices of at most kSliceValues values (a longer block is a slice by itself), slices and rows to
-// warps.  A warp's share of the grid is its slice's length; with few rows a stage holds fewer of them, so that they spread over the SMs.
-// Rows that are dense but no multiple of 16 bytes come in stages of 2, 4 or 8, which are.
+// Divides the work: neighbouring irrep blocks to slices of at most kSliceValues values (a longer block is a slice by itself); the warps that
+// shared memory and registers hold at a time share the rows of every slice.  (Warps of one slice each, in proportion to its length,
+// were 35 % idle in the end: no length says what a slice costs.)  Rows that are dense but no multiple of 16 bytes come in stages of 2, 4 or 8, which are.
 int make_plan(const cueq_norm_args* a, bool backward, bool dense, Params* p, int* grid, int* smem_bytes) {
   const bool q8 = a->codes != nullptr;
   const int size = element_size(a->dtype), msize = a->dtype == CUEQ_F64 ? 8 : 4, stat = p->ns * msize;
-  int64_t total = 0;
   int ns = 0;
   bool even = true;
   for (int k = 0; k < a->num_blocks; ++k) {
@@ -121,6 +119,8 @@ int make_plan(const cueq_norm_args* a, bool backward, bool dense, Params* p, int
   auto stage = [&](const Slice& s) { return backward ? backward_stage(*p, s, a->mode, q8, size, stat).total : forward_stage(*p, s, a->mode, q8, size).total; };
   auto need = [&](const Slice& s, int stages) { return head_bytes(msize, s.channels, backward) + stages * stage(s); };
   p->stages = 2;
+  p->unit = unit;
+  int smem = 0;
   for (int k = 0; k < ns; ++k) {
     Slice& s = p->slice[k];
     s.rps = unit;
@@ -130,33 +130,14 @@ int make_plan(const cueq_norm_args* a, bool backward, bool dense, Params* p, int
     int rps = kStageBytes / (one ? one : 1) / unit * unit;
     s.rps = rps < unit ? unit : rps > 32 ? 32 : rps;
     while (s.rps > unit && copy_lanes(a, backward, *p, s.rps) > 32) s.rps -= unit;
-    total += s.values + kItemCost * s.count;
   }
-  // fewer rows per stage where that lets each warp of a full GPU have some
-  int smem = 0;
   for (int k = 0; k < ns; ++k) { const int b = need(p->slice[k], p->stages); smem = b > smem ? b : smem; }
   *smem_bytes = smem;
   if (smem > kSmemPerSm) return kTooLong;
   int occupancy = kSmemPerSm / (smem + 1024);
-  occupancy = occupancy > warps_per_sm(msize) ? warps_per_sm(msize) : occupancy;
-  const int64_t warps = (int64_t)kSms * (occupancy < 1 ? 1 : occupancy);
-  int at = 0;
-  int64_t part = 0;
-  for (int k = 0; k < ns; ++k) {
-    Slice& s = p->slice[k];
-    int64_t share = warps * (s.values + kItemCost * s.count) / total;
-    share = share < 1 ? 1 : share;
-    const int64_t spread = a->rows / share / unit * unit;
-    if (s.rps > spread) s.rps = spread < unit ? unit : (int)spread;
-    const int64_t units = (a->rows + s.rps - 1) / s.rps;
-    s.ncta = (int)(share < units ? share : units);
-    s.cta0 = at;
-    at += s.ncta;
-    s.part = part;
-    part += (int64_t)s.ncta * s.channels;
-  }
-  p->parts_len = part;
-  *grid = at;
+  occupancy = occupancy < 1 ? 1 : occupancy > warps_per_sm(msize) ? warps_per_sm(msize) : occupancy;
+  const int64_t units = (a->rows + unit - 1) / unit * ns, warps = (int64_t)kSms * occupancy;
+  *grid = (int)(units < warps ? units : warps);
   return 0;
 }
 
@@ -178,10 +159,8 @@ int fill(const cueq_norm_args* a, bool backward, Params* p, int* grid, int* smem
 // dscale, dweight: the warps' sums of a channel, in order
 struct SumParams {
   const void* parts;
-  int64_t parts_len;
   void* out[2];
-  int num_slices, channels, dtype;
-  struct { int channels, ch, ncta; int64_t part; } slice[kMaxBlocks];
+  int warps, channels, dtype;
 };
 constexpr int kSumRows = 32;
 template <class M>
@@ -191,11 +170,9 @@ __global__ void __launch_bounds__(32 * kSumRows) sum_kernel(const __grid_constan
   const int which = blockIdx.y;
   M v = M(0);
   if (ch < p.channels && p.out[which]) {
-    int k = 0;
-    while (k + 1 < p.num_slices && ch >= p.slice[k + 1].ch) ++k;
-    const M* src = reinterpret_cast<const M*>(p.parts) + which * p.parts_len + p.slice[k].part + (ch - p.slice[k].ch);
+    const M* src = reinterpret_cast<const M*>(p.parts) + (int64_t)which * p.warps * p.channels + ch;
 #pragma unroll 8
-    for (int j = threadIdx.y; j < p.slice[k].ncta; j += kSumRows) v += src[(int64_t)j * p.slice[k].channels];
+    for (int j = threadIdx.y; j < p.warps; j += kSumRows) v += src[(int64_t)j * p.channels];
   }
   partial[threadIdx.y][threadIdx.x] = v;
   __syncthreads();
@@ -242,7 +219,7 @@ int launch(const cueq_norm_args* a, bool backward, void* stream) {
     if (norm ? !operand(a->gn, a->ldgn, width) : !operand(a->go, a->ldgo, width)) return cueq::fail("norm: a cotangent is missing or its rows overlap");
     if (a->mode == kBoth && a->go && !operand(a->go, a->ldgo, width)) return cueq::fail("norm: a cotangent's rows overlap");
     if ((branch && !a->dy) || (norm && !a->dx) || (gated(a) && !a->dg)) return cueq::fail("norm: null result");
-    const int64_t need = 2 * p.parts_len;
+    const int64_t need = 2 * (int64_t)grid * p.channels;
     if (a->rows && (!a->parts || a->parts_values < need)) return cueq::fail("norm: the parameters' gradients need room for %lld partial sums", (long long)need);
   }
   p.x = a->x; p.y = a->y; p.g = a->g; p.h = a->h; p.go = a->go; p.gn = a->gn;
@@ -266,17 +243,8 @@ int launch(const cueq_norm_args* a, bool backward, void* stream) {
     CUEQ_CUDA_OK(cudaGetLastError());
   }
   if (!backward) return 0;
-  SumParams s;
-  std::memset(&s, 0, sizeof(s));
-  s.parts = a->parts; s.parts_len = p.parts_len;
-  s.out[0] = branch ? a->dscale : nullptr;
-  s.out[1] = norm ? a->dweight : nullptr;
+  SumParams s{a->parts, {branch ? a->dscale : nullptr, norm ? a->dweight : nullptr}, a->rows ? grid : 0, p.channels, a->param_dtype};
   if (!s.out[0] && !s.out[1]) return 0;
-  s.num_slices = p.num_slices; s.channels = p.channels; s.dtype = a->param_dtype;
-  for (int k = 0; k < p.num_slices; ++k) {
-    const Slice& q = p.slice[k];
-    s.slice[k].channels = q.channels; s.slice[k].ch = p.blk[q.first].ch; s.slice[k].ncta = a->rows ? q.ncta : 0; s.slice[k].part = q.part;
-  }
   const dim3 g((p.channels + 31) / 32, 2), t(32, kSumRows);
   if (a->dtype == CUEQ_F64) sum_kernel<double><<<g, t, 0, st>>>(s);
   else sum_kernel<float><<<g, t, 0, st>>>(s);
@@ -291,7 +259,7 @@ extern "C" int64_t cueq_b200_norm_stats(const cueq_norm_args* a) { return check(
 extern "C" int64_t cueq_b200_norm_parts(const cueq_norm_args* a) {
   Params p;
   int grid, smem;
-  return fill(a, true, &p, &grid, &smem) ? -1 : 2 * p.parts_len;
+  return fill(a, true, &p, &grid, &smem) ? -1 : 2 * (int64_t)grid * p.channels;
 }
 extern "C" int cueq_b200_norm_forward(const cueq_norm_args* a, void* stream) { return launch(a, false, stream); }
 extern "C" int cueq_b200_norm_backward(const cueq_norm_args* a, void* stream) { return launch(a, true, stream); }

@@ -46,8 +46,7 @@ struct Blk {
 struct Slice {
   int first, count;                  // blocks
   int values, channels;              // their elements and channels
-  int cta0, ncta, rps;               // thread blocks, rows per stage
-  int64_t part;                      // first partial sum
+  int rps;                           // rows per stage
 };
 // How rows of an operand move.  kRows: a bulk copy per row; kDense: rows follow one another without a gap, one bulk copy per stage;
 // kPlain: element by element, where addresses or lengths are not multiples of 16 bytes.
@@ -64,12 +63,11 @@ struct Params {
   int64_t ldc;
   void* stats;
   void* parts;
-  int64_t parts_len;                 // of one of the two gradients
   int64_t rows;
   double eps;
   int* status;
   int nb, ns, dim_total, channels;   // ns: statistics per (row, block)
-  int num_slices, stages;            // stages: 2, or 1 where two do not fit into shared memory
+  int num_slices, unit, stages;      // unit: rows after which dense rows are on a 16-byte boundary again; stages: 2, or 1 where two do not fit into shared memory
   int pdtype, gate, mul_ir;
   signed char route[kTensors];
   Blk blk[kMaxBlocks];
@@ -331,31 +329,30 @@ __device__ __forceinline__ void backward_item(const View<M>& c, T* __restrict__ 
   }
 }
 
-// ---- one (row, irrep block) of at most 128 channels: a lane's K channels in registers ------------------------------------------------
-// Read from shared memory once, written once.  32 K is the number of channels or above it.
+// ---- one (row, irrep block) of 32 K channels, K <= 4, in registers ------------------------------------------------
+// Read from shared memory once, written once.
 template <class T, class M, int DIM, bool MUL_IR, int K>
 struct Short {
   int lane, mul;
-  __device__ __forceinline__ bool ok(int k) const { return lane + 32 * k < mul; }
   __device__ __forceinline__ int at(int k, int i) const { return MUL_IR ? (lane + 32 * k) * DIM + i : i * mul + lane + 32 * k; }
   template <class E>
   __device__ __forceinline__ void load(const E* p, M (&v)[K][DIM]) const {
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < DIM; ++i) v[k][i] = ok(k) ? to<M>(p[at(k, i)]) : M(0);
+      for (int i = 0; i < DIM; ++i) v[k][i] = to<M>(p[at(k, i)]);
   }
   __device__ __forceinline__ void store(T* p, const M (&v)[K][DIM]) const {
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < DIM; ++i) if (ok(k)) p[at(k, i)] = from<T>(v[k][i]);
+      for (int i = 0; i < DIM; ++i) p[at(k, i)] = from<T>(v[k][i]);
   }
   __device__ __forceinline__ void store_codes(signed char* p, const M (&v)[K][DIM], float inverse) const {
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int i = 0; i < DIM; ++i) if (ok(k)) p[at(k, i)] = to_code(v[k][i], inverse);
+      for (int i = 0; i < DIM; ++i) p[at(k, i)] = to_code(v[k][i], inverse);
   }
   __device__ __forceinline__ M squares(const M (&v)[K][DIM]) const {
     M part[DIM];
@@ -387,14 +384,14 @@ __device__ __forceinline__ void forward_short(const View<M>& c, T* x, T* y, cons
   M xv[K][DIM];
   if (MODE & kBranch) q.load(x, xv);
 #pragma unroll
-  for (int k = 0; k < K; ++k) a[k] = q.ok(k) ? ((MODE & kBranch) ? c.s : c.w)[c.lane + 32 * k] : M(0);
+  for (int k = 0; k < K; ++k) a[k] = ((MODE & kBranch) ? c.s : c.w)[c.lane + 32 * k];
   float gstep = 0.f, ginv = 0.f;
   if ((MODE & kBranch) && c.gated) {
     M gate[K];
     unsigned gtop = 0;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      gate[k] = q.ok(k) ? to<M>(g[c.lane + 32 * k]) : M(0);
+      gate[k] = to<M>(g[c.lane + 32 * k]);
       if (Q8) gtop = max(gtop, magnitude(gate[k]));
     }
     if (Q8) code_step(__reduce_max_sync(0xffffffffu, gtop), gstep, ginv);
@@ -403,7 +400,7 @@ __device__ __forceinline__ void forward_short(const View<M>& c, T* x, T* y, cons
       M e, de;
       activation(c.gate, gate[k], e, de);
       a[k] *= e;
-      if (Q8 && q.ok(k)) cg[c.lane + 32 * k] = to_code(gate[k], ginv);
+      if (Q8) cg[c.lane + 32 * k] = to_code(gate[k], ginv);
     }
   }
   const M r = inverse_sqrt(cueq::warp_sum(q.squares(v)) * c.inv_n + c.eps);
@@ -427,7 +424,7 @@ __device__ __forceinline__ void forward_short(const View<M>& c, T* x, T* y, cons
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const M b = q.ok(k) ? c.w[c.lane + 32 * k] * rh : M(0);
+      const M b = c.w[c.lane + 32 * k] * rh;
 #pragma unroll
       for (int i = 0; i < DIM; ++i) v[k][i] *= b;
     }
@@ -454,8 +451,8 @@ __device__ __forceinline__ void backward_short(const View<M>& c, T* go, T* gn, c
 #pragma unroll
       for (int i = 0; i < DIM; ++i) p += o[k][i] * v[k][i];
       p *= rh * step;
-      b[k] = q.ok(k) ? c.w[c.lane + 32 * k] : M(0);
-      if (q.ok(k)) c.acc_w[c.lane + 32 * k] += p;
+      b[k] = c.w[c.lane + 32 * k];
+      c.acc_w[c.lane + 32 * k] += p;
       dot += b[k] * p;
     }
     const M qh = rh * (rh * (c.inv_n * cueq::warp_sum(dot))) * step;
@@ -485,17 +482,15 @@ __device__ __forceinline__ void backward_short(const View<M>& c, T* go, T* gn, c
   for (int k = 0; k < K; ++k) {
     const int u = c.lane + 32 * k;
     M e = M(1), de = M(0), p = M(0);
-    if (c.gated) activation(c.gate, q.ok(k) ? to<M>(g[u]) * gstep : M(0), e, de);
+    if (c.gated) activation(c.gate, to<M>(g[u]) * gstep, e, de);
 #pragma unroll
     for (int i = 0; i < DIM; ++i) p += o[k][i] * v[k][i];
     p *= r * step;
-    const M s = q.ok(k) ? c.s[u] : M(0);
+    const M s = c.s[u];
     a[k] = s * e;
     dot += a[k] * p;
-    if (q.ok(k)) {
-      c.acc_s[u] += e * p;
-      if (c.gated) dg[u] = from<T>(s * de * p);          // may lie over g[u]
-    }
+    c.acc_s[u] += e * p;
+    if (c.gated) dg[u] = from<T>(s * de * p);            // may lie over g[u]
   }
   const M qy = r * (r * (c.inv_n * cueq::warp_sum(dot))) * step;
 #pragma unroll
@@ -577,9 +572,10 @@ __device__ __forceinline__ unsigned job_bytes(const Job& j, int n) { return j.ro
 
 // Rows first .. last in stages of rps rows; `work(stage, z, n)`.  A lane that issues loads into a stage waits for its own stores out of
 // it; the warp then meets, so that no lane's load overtakes another lane's store.  One stage at a time where two do not fit.
-template <class Work>
-__device__ __forceinline__ void run_stages(const Params& p, int rps, int64_t first, int64_t last, const Move* in, int nin, const Move* out, int nout,
-                                           unsigned char* stages, int stage_bytes, unsigned long long* full, Work work) {
+// `ready()` runs while the first loads are under way.  `phases`, bit s: the phase that stage s waits for.  False: given up.
+template <class Ready, class Work>
+__device__ __forceinline__ bool run_stages(const Params& p, int rps, int64_t first, int64_t last, const Move* in, int nin, const Move* out, int nout,
+                                           unsigned char* stages, int stage_bytes, unsigned long long* full, unsigned& phases, Ready ready, Work work) {
   const int lane = threadIdx.x;
   Job jin = make_job(in, nin, rps, first), jout = make_job(out, nout, rps, first);
   auto load = [&](int64_t z, int s) {
@@ -594,8 +590,8 @@ __device__ __forceinline__ void run_stages(const Params& p, int rps, int64_t fir
   };
   const bool two = p.stages == 2;
   if (first < last) load(first, 0);
+  ready();
   int s = 0;
-  unsigned phases = 0;                                   // bit s: the phase that stage s waits for
   for (int64_t z = first; z < last; z += rps) {
     const int n = (int)min((int64_t)rps, last - z);
     const bool more = z + rps < last;
@@ -607,7 +603,7 @@ __device__ __forceinline__ void run_stages(const Params& p, int rps, int64_t fir
     if (!__all_sync(0xffffffffu, bar_wait(full + s, phases >> s & 1, p.status))) {   // a copy did not arrive in time: give up once those in flight have landed
       if (two && more) bar_wait(full + (s ^ 1), phases >> (s ^ 1) & 1, p.status);
       bar_wait(full + s, phases >> s & 1, p.status);
-      break;
+      return false;
     }
     phases ^= 1u << s;
     unsigned char* stage = stages + s * stage_bytes;
@@ -627,30 +623,36 @@ __device__ __forceinline__ void run_stages(const Params& p, int rps, int64_t fir
     }
   }
   asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
+  __syncwarp();
+  return true;
 }
 
-__device__ __forceinline__ const Slice& my_slice(const Params& p) {
-  int k = 0;
-  while (k + 1 < p.num_slices && (int)blockIdx.x >= p.slice[k + 1].cta0) ++k;
-  return p.slice[k];
+// The rows of slice s for this warp.  Units of rows are dealt out row by row, all slices of one before the next, in equal numbers: every
+// warp has its share of every slice, whatever a slice costs.
+__device__ __forceinline__ void my_rows(const Params& p, int s, int64_t& first, int64_t& last) {
+  const int64_t total = (p.rows + p.unit - 1) / p.unit * p.num_slices;
+  const int64_t a = total * blockIdx.x / gridDim.x, b = total * (blockIdx.x + 1) / gridDim.x;
+  first = (a - s + p.num_slices - 1) / p.num_slices * p.unit;
+  last = min(p.rows, (b - s + p.num_slices - 1) / p.num_slices * p.unit);
 }
-// parameters of the slice's channels into shared memory, sums cleared, barriers
-template <class M>
-__device__ __forceinline__ M* prepare(const Params& p, const Slice& s, unsigned char* smem, bool backward) {
-  M* at = reinterpret_cast<M*>(smem + kBars);
-  const int ch = p.blk[s.first].ch, n = s.channels;
-  for (int u = threadIdx.x; u < n; u += 32) {
-    at[u] = p.s ? cueq::load_as<M>(p.s, p.pdtype, ch + u) : M(1);
-    at[n + u] = p.w ? cueq::load_as<M>(p.w, p.pdtype, ch + u) : M(1);
-    if (backward) at[3 * n + u] = at[4 * n + u] = M(0);
-  }
+__device__ __forceinline__ void init_barriers(unsigned char* smem) {
   if (threadIdx.x == 0) {
     bar_init(reinterpret_cast<unsigned long long*>(smem), 1);
     bar_init(reinterpret_cast<unsigned long long*>(smem) + 1, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   __syncwarp();
-  return at;
+}
+// parameters of the slice's channels into shared memory, sums cleared
+template <class M>
+__device__ __forceinline__ void prepare(const Params& p, const Slice& s, M* at, bool backward) {
+  const int ch = p.blk[s.first].ch, n = s.channels;
+  for (int u = threadIdx.x; u < n; u += 32) {
+    at[u] = p.s ? cueq::load_as<M>(p.s, p.pdtype, ch + u) : M(1);
+    at[n + u] = p.w ? cueq::load_as<M>(p.w, p.pdtype, ch + u) : M(1);
+    if (backward) at[3 * n + u] = at[4 * n + u] = M(0);
+  }
+  __syncwarp();
 }
 template <class M>
 __device__ __forceinline__ View<M> block_view(const Params& p, const Slice& s, const Blk& b, M* at) {
@@ -677,9 +679,9 @@ __device__ __forceinline__ void put_moves(Move* moves, const Move (&in)[NIN], in
 }
 
 // (dimension, channels per lane) of a block: CALL for those that registers hold, LONG for the others
-#define CUEQ_NORM_K(D, CALL) if (b.mul <= 32) CALL(D, 1); else if (b.mul <= 64) CALL(D, 2); else CALL(D, 4)
+#define CUEQ_NORM_K(D, CALL) if (b.mul == 32) CALL(D, 1); else if (b.mul == 64) CALL(D, 2); else if (b.mul == 96) CALL(D, 3); else CALL(D, 4)
 #define CUEQ_NORM_DIMS(CALL, LONG)                                                     \
-  if (b.mul <= 128 && b.dim <= 7) {                                                    \
+  if (b.mul <= 128 && b.mul % 32 == 0 && b.dim <= 7) {                                                    \
     switch (b.dim) {                                                                   \
       case 1: CUEQ_NORM_K(1, CALL); break;                                             \
       case 3: CUEQ_NORM_K(3, CALL); break;                                             \
@@ -697,13 +699,9 @@ __device__ __forceinline__ void put_moves(Move* moves, const Move (&in)[NIN], in
   }
 
 template <class T, class M, int MODE, bool Q8, bool MUL_IR>
-__global__ void __launch_bounds__(32, warps_per_sm(sizeof(M))) forward_kernel(const __grid_constant__ Params p) {
-  extern __shared__ __align__(128) unsigned char smem[];
-  const Slice& sl = my_slice(p);
-  M* at = prepare<M>(p, sl, smem, false);
+__device__ __forceinline__ bool forward_slice(const Params& p, const Slice& sl, int64_t first, int64_t last, unsigned char* smem, unsigned& phases) {
+  M* at = reinterpret_cast<M*>(smem + kBars);
   constexpr int size = sizeof(T);
-  const int64_t units = (p.rows + sl.rps - 1) / sl.rps, j = blockIdx.x - sl.cta0;
-  const int64_t first = units * j / sl.ncta * sl.rps, last = min(p.rows, units * (j + 1) / sl.ncta * sl.rps);
   const Stage st = forward_stage(p, sl, MODE, Q8, size);
   const Blk& b0 = p.blk[sl.first];
   const bool gated = (MODE & kBranch) && p.gate != CUEQ_NORM_GATE_NONE;
@@ -723,8 +721,8 @@ __global__ void __launch_bounds__(32, warps_per_sm(sizeof(M))) forward_kernel(co
   const int nout = 1 + (MODE == kBoth) + (Q8 ? 1 + (MODE == kBoth) + gated : 0);
   const int nin = (MODE & kBranch) ? 2 + gated : 1;
   put_moves(moves, in, nin, out, nout);
-  run_stages(p, sl.rps, first, last, moves, nin, moves + nin, nout, smem + head_bytes(sizeof(M), sl.channels, false), st.total,
-             reinterpret_cast<unsigned long long*>(smem), [&](unsigned char* s, int64_t z, int n) {
+  return run_stages(p, sl.rps, first, last, moves, nin, moves + nin, nout, smem + head_bytes(sizeof(M), sl.channels, false), st.total,
+                    reinterpret_cast<unsigned long long*>(smem), phases, [&]() { prepare<M>(p, sl, at, false); }, [&](unsigned char* s, int64_t z, int n) {
     for (int k = sl.first; k < sl.first + sl.count; ++k) {
       const Blk& b = p.blk[k];
       const View<M> c = block_view<M>(p, sl, b, at);
@@ -750,15 +748,11 @@ template <class T, bool Q8> struct Kept { using type = T; };
 template <class T> struct Kept<T, true> { using type = signed char; };
 
 template <class T, class M, int MODE, bool Q8, bool MUL_IR>
-__global__ void __launch_bounds__(32, warps_per_sm(sizeof(M))) backward_kernel(const __grid_constant__ Params p) {
+__device__ __forceinline__ bool backward_slice(const Params& p, const Slice& sl, int64_t first, int64_t last, unsigned char* smem, unsigned& phases) {
   using K = typename Kept<T, Q8>::type;
-  extern __shared__ __align__(128) unsigned char smem[];
-  const Slice& sl = my_slice(p);
-  M* at = prepare<M>(p, sl, smem, true);
+  M* at = reinterpret_cast<M*>(smem + kBars);
   constexpr int size = sizeof(T);
   const int stat = p.ns * (int)sizeof(M);
-  const int64_t units = (p.rows + sl.rps - 1) / sl.rps, j = blockIdx.x - sl.cta0;
-  const int64_t first = units * j / sl.ncta * sl.rps, last = min(p.rows, units * (j + 1) / sl.ncta * sl.rps);
   const Stage st = backward_stage(p, sl, MODE, Q8, size, stat);
   const Blk& b0 = p.blk[sl.first];
   const bool branch = MODE & kBranch, gated = branch && p.gate != CUEQ_NORM_GATE_NONE, has_go = p.go != nullptr;
@@ -782,8 +776,8 @@ __global__ void __launch_bounds__(32, warps_per_sm(sizeof(M))) backward_kernel(c
   const Move out[3] = {MODE == kNorm ? o_b : o_a, MODE == kBoth ? o_b : o_g, o_g};
   const int nout = MODE == kNorm ? 1 : 1 + (MODE == kBoth) + gated;
   put_moves(moves, in, nin, out, nout);
-  run_stages(p, sl.rps, first, last, moves, nin, moves + nin, nout, smem + head_bytes(sizeof(M), sl.channels, true), st.total,
-             reinterpret_cast<unsigned long long*>(smem), [&](unsigned char* s, int64_t, int n) {
+  const bool done = run_stages(p, sl.rps, first, last, moves, nin, moves + nin, nout, smem + head_bytes(sizeof(M), sl.channels, true), st.total,
+                               reinterpret_cast<unsigned long long*>(smem), phases, [&]() { prepare<M>(p, sl, at, true); }, [&](unsigned char* s, int64_t, int n) {
     for (int k = sl.first; k < sl.first + sl.count; ++k) {
       const Blk& b = p.blk[k];
       const View<M> c = block_view<M>(p, sl, b, at);
@@ -804,10 +798,37 @@ __global__ void __launch_bounds__(32, warps_per_sm(sizeof(M))) backward_kernel(c
     }
   });
   // this warp's sums of the parameters' gradients
-  M* dst = reinterpret_cast<M*>(p.parts) + sl.part + j * sl.channels;
+  M* dst = reinterpret_cast<M*>(p.parts) + (int64_t)blockIdx.x * p.channels + b0.ch;
   for (int u = threadIdx.x; u < sl.channels; u += 32) {
     if (MODE & kBranch) dst[u] = at[3 * sl.channels + u];
-    if (MODE & kNorm) dst[p.parts_len + u] = at[4 * sl.channels + u];
+    if (MODE & kNorm) dst[(int64_t)gridDim.x * p.channels + u] = at[4 * sl.channels + u];
+  }
+  __syncwarp();
+  return done;
+}
+
+template <class T, class M, int MODE, bool Q8, bool MUL_IR>
+__global__ void __launch_bounds__(32, warps_per_sm(sizeof(M))) forward_kernel(const __grid_constant__ Params p) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  init_barriers(smem);
+  unsigned phases = 0;
+  for (int k = 0; k < p.num_slices; ++k) {               // neighbouring warps start with different slices
+    const int s = (k + blockIdx.x) % p.num_slices;
+    int64_t first, last;
+    my_rows(p, s, first, last);
+    if (first < last && !forward_slice<T, M, MODE, Q8, MUL_IR>(p, p.slice[s], first, last, smem, phases)) return;
+  }
+}
+template <class T, class M, int MODE, bool Q8, bool MUL_IR>
+__global__ void __launch_bounds__(32, warps_per_sm(sizeof(M))) backward_kernel(const __grid_constant__ Params p) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  init_barriers(smem);
+  unsigned phases = 0;
+  for (int k = 0; k < p.num_slices; ++k) {
+    const int s = (k + blockIdx.x) % p.num_slices;
+    int64_t first, last;
+    my_rows(p, s, first, last);
+    if (!backward_slice<T, M, MODE, Q8, MUL_IR>(p, p.slice[s], first, last, smem, phases)) return;
   }
 }
 
