@@ -104,7 +104,6 @@ int make_plan(const cueq_norm_args* a, bool backward, bool dense, Params* p, int
     b.mul = a->blocks[k].mul; b.dim = a->blocks[k].dim;
     b.off = p->dim_total; b.ch = p->channels;
     const int n = b.mul * b.dim;
-    b.inv_n = 1.0 / n;
     if (!ns || p->slice[ns - 1].values + n > kSliceValues) { p->slice[ns] = Slice{}; p->slice[ns].first = k; ++ns; }
     Slice& s = p->slice[ns - 1];
     if (s.count == 0 && (b.off * size % 16 || (gated(a) && b.ch * size % 16))) even = false;
@@ -128,6 +127,7 @@ int make_plan(const cueq_norm_args* a, bool backward, bool dense, Params* p, int
     if (need(s, 2) > kSmemPerSm) p->stages = 1;
     const int one = stage(s) / unit;
     int rps = kStageBytes / (one ? one : 1) / unit * unit;
+    rps = rps >= 3 ? (rps + 1) & ~3 : rps;               // rows are worked on by fours, twos or one by one
     s.rps = rps < unit ? unit : rps > 32 ? 32 : rps;
     while (s.rps > unit && copy_lanes(a, backward, *p, s.rps) > 32) s.rps -= unit;
   }

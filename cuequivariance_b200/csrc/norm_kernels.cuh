@@ -33,6 +33,7 @@ using cueq_tc::bar_init;
 using cueq_tc::bar_wait;
 using cueq_tc::s32;
 
+// Params stay below 4 KB
 constexpr int kMaxBlocks = CUEQ_NORM_MAX_BLOCKS;
 // warps of an SM that its registers hold
 __host__ __device__ constexpr int warps_per_sm(int msize) { return msize == 8 ? 8 : 16; }
@@ -40,7 +41,6 @@ enum Mode { kBranch = 1, kNorm = 2, kBoth = 3 };
 
 struct Blk {
   int mul, dim, off, ch;             // off, ch: first element of the block in a row of features, first channel
-  double inv_n;                      // 1 / (mul dim)
   int code, gcode, hcode;            // first byte in a row of codes: of y (or x, norm alone), of the gates, of h
 };
 struct Slice {
@@ -74,6 +74,7 @@ struct Params {
   Slice slice[kMaxBlocks];
 };
 
+static_assert(sizeof(Params) <= 4000, "kernel parameters");
 __host__ __device__ constexpr int pad16(int bytes) { return (bytes + 15) & ~15; }
 __host__ __device__ inline int code_bytes(const Params& p, const Slice& s) {
   int n = 0;
@@ -329,175 +330,286 @@ __device__ __forceinline__ void backward_item(const View<M>& c, T* __restrict__ 
   }
 }
 
-// ---- one (row, irrep block) of 32 K channels, K <= 4, in registers ------------------------------------------------
-// Read from shared memory once, written once.
-template <class T, class M, int DIM, bool MUL_IR, int K>
-struct Short {
-  int lane, mul;
-  __device__ __forceinline__ int at(int k, int i) const { return MUL_IR ? (lane + 32 * k) * DIM + i : i * mul + lane + 32 * k; }
-  template <class E>
-  __device__ __forceinline__ void load(const E* p, M (&v)[K][DIM]) const {
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < DIM; ++i) v[k][i] = to<M>(p[at(k, i)]);
-  }
-  __device__ __forceinline__ void store(T* p, const M (&v)[K][DIM]) const {
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < DIM; ++i) p[at(k, i)] = from<T>(v[k][i]);
-  }
-  __device__ __forceinline__ void store_codes(signed char* p, const M (&v)[K][DIM], float inverse) const {
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < DIM; ++i) p[at(k, i)] = to_code(v[k][i], inverse);
-  }
-  __device__ __forceinline__ M squares(const M (&v)[K][DIM]) const {
-    M part[DIM];
-#pragma unroll
-    for (int i = 0; i < DIM; ++i) part[i] = v[0][i] * v[0][i];
-#pragma unroll
-    for (int k = 1; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < DIM; ++i) part[i] += v[k][i] * v[k][i];
-#pragma unroll
-    for (int i = 1; i < DIM; ++i) part[0] += part[i];
-    return part[0];
-  }
-  __device__ __forceinline__ unsigned top(const M (&v)[K][DIM]) const {
-    unsigned t = 0;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < DIM; ++i) t = max(t, magnitude(v[k][i]));
-    return __reduce_max_sync(0xffffffffu, t);
-  }
+// ---- R rows of one irrep block of 32 K channels, K <= 4, in registers -----------------------------------------------------------------
+// Read from shared memory once, written once.  Short blocks take several rows at a time: what a call costs besides its values, above all the
+// sums over the warp, is most of their time.  Of fewer than R rows the last one is read in place of the missing ones.
+template <int DIM, int K> constexpr int kRowsAtOnce = DIM * K <= 2 ? 4 : DIM * K <= 8 ? 2 : 1;
+
+// rows of one region: E at byte `base`, `pitch` bytes apart
+template <class E>
+struct Rows {
+  unsigned char* base;
+  int pitch;
+  __device__ __forceinline__ E* operator[](int q) const { return reinterpret_cast<E*>(base + q * pitch); }
 };
 
-template <class T, class M, int MODE, bool Q8, int DIM, bool MUL_IR, int K>
-__device__ __forceinline__ void forward_short(const View<M>& c, T* x, T* y, const T* g, signed char* ca, signed char* cg, signed char* ch, M* stats) {
-  const Short<T, M, DIM, MUL_IR, K> q{c.lane, c.mul};
-  M v[K][DIM], a[K];
-  q.load((MODE & kBranch) ? y : x, v);
-  M xv[K][DIM];
-  if (MODE & kBranch) q.load(x, xv);
-#pragma unroll
-  for (int k = 0; k < K; ++k) a[k] = ((MODE & kBranch) ? c.s : c.w)[c.lane + 32 * k];
-  float gstep = 0.f, ginv = 0.f;
-  if ((MODE & kBranch) && c.gated) {
-    M gate[K];
-    unsigned gtop = 0;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      gate[k] = to<M>(g[c.lane + 32 * k]);
-      if (Q8) gtop = max(gtop, magnitude(gate[k]));
-    }
-    if (Q8) code_step(__reduce_max_sync(0xffffffffu, gtop), gstep, ginv);
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      M e, de;
-      activation(c.gate, gate[k], e, de);
-      a[k] *= e;
-      if (Q8) cg[c.lane + 32 * k] = to_code(gate[k], ginv);
-    }
-  }
-  const M r = inverse_sqrt(cueq::warp_sum(q.squares(v)) * c.inv_n + c.eps);
-  float step = 0.f, inv = 0.f;
-  if (Q8) {
-    code_step(q.top(v), step, inv);
-    q.store_codes(ca, v, inv);
-  }
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int i = 0; i < DIM; ++i) v[k][i] = (MODE & kBranch) ? xv[k][i] + a[k] * r * v[k][i] : a[k] * r * v[k][i];
-  q.store(x, v);
-  M rh = M(0);
-  float hstep = 0.f, hinv = 0.f;
-  if (MODE == kBoth) {
-    rh = inverse_sqrt(cueq::warp_sum(q.squares(v)) * c.inv_n + c.eps);
-    if (Q8) {
-      code_step(q.top(v), hstep, hinv);
-      q.store_codes(ch, v, hinv);
+// sums of R values each over the warp, every one by the same pairs in the same order as cueq::warp_sum
+template <int R, class M>
+__device__ __forceinline__ void warp_sums(M (&s)[R], int lane) {
+  if constexpr (R == 1) {
+    s[0] = cueq::warp_sum(s[0]);
+  } else {
+    constexpr unsigned all = 0xffffffffu;
+    M t;
+    if constexpr (R == 2) {
+      const bool up = lane & 16;
+      t = (up ? s[1] : s[0]) + __shfl_xor_sync(all, up ? s[0] : s[1], 16);
+      t += __shfl_xor_sync(all, t, 8);
+    } else {
+      const bool up = lane & 16, odd = lane & 8;
+      const M a = (up ? s[1] : s[0]) + __shfl_xor_sync(all, up ? s[0] : s[1], 16), b = (up ? s[3] : s[2]) + __shfl_xor_sync(all, up ? s[2] : s[3], 16);
+      t = (odd ? b : a) + __shfl_xor_sync(all, odd ? a : b, 8);
     }
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const M b = c.w[c.lane + 32 * k] * rh;
+    for (int o = 4; o; o >>= 1) t += __shfl_xor_sync(all, t, o);
 #pragma unroll
-      for (int i = 0; i < DIM; ++i) v[k][i] *= b;
-    }
-    q.store(y, v);
-  }
-  if (stats && c.lane == 0) {
-    stats[0] = r; stats[1] = rh; stats[2] = M(step); stats[3] = M(gstep);
-    if (Q8 && MODE == kBoth) stats[4] = M(hstep);
+    for (int q = 0; q < R; ++q) s[q] = __shfl_sync(all, t, (q & 1) * 16 + (q >> 1) * 8);
   }
 }
 
-template <class T, class M, class K8, int MODE, bool Q8, int DIM, bool MUL_IR, int K>
-__device__ __forceinline__ void backward_short(const View<M>& c, T* go, T* gn, const K8* h, const K8* y, const K8* g, T* dg, const M* stats, bool has_go) {
-  const Short<T, M, DIM, MUL_IR, K> q{c.lane, c.mul};
-  M o[K][DIM], v[K][DIM];
-  if (MODE & kNorm) {
-    const M rh = stats[MODE == kBoth ? 1 : 0], step = Q8 ? stats[MODE == kBoth ? 4 : 2] : M(1);
-    q.load(gn, o);
-    q.load(h, v);
-    M dot = M(0), b[K];
+template <class T, class M, int DIM, bool MUL_IR, int K, int R>
+struct Short {
+  int lane, mul, left;               // left: rows that there are, 1 .. R
+  __device__ __forceinline__ int row(int q) const { return R == 1 ? 0 : min(q, left - 1); }
+  __device__ __forceinline__ bool there(int q) const { return R == 1 || q < left; }
+  __device__ __forceinline__ int at(int k, int i) const { return MUL_IR ? (lane + 32 * k) * DIM + i : i * mul + lane + 32 * k; }
+  template <class E>
+  __device__ __forceinline__ void load(const Rows<E>& p, M (&v)[R][K][DIM]) const {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      M p = M(0);
-#pragma unroll
-      for (int i = 0; i < DIM; ++i) p += o[k][i] * v[k][i];
-      p *= rh * step;
-      b[k] = c.w[c.lane + 32 * k];
-      c.acc_w[c.lane + 32 * k] += p;
-      dot += b[k] * p;
-    }
-    const M qh = rh * (rh * (c.inv_n * cueq::warp_sum(dot))) * step;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int i = 0; i < DIM; ++i) o[k][i] = b[k] * rh * o[k][i] - qh * v[k][i];
-    if (MODE == kNorm) {
-      q.store(gn, o);
-      return;
-    }
-    if (has_go) {
-      q.load(go, v);
+    for (int q = 0; q < R; ++q) {
+      const E* e = p[row(q)];
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < DIM; ++i) o[k][i] += v[k][i];
+        for (int i = 0; i < DIM; ++i) v[q][k][i] = to<M>(e[at(k, i)]);
     }
-    q.store(go, o);
-  } else {
-    q.load(go, o);
   }
-  const M r = stats[0], step = Q8 ? stats[2] : M(1), gstep = Q8 ? stats[3] : M(1);
-  q.load(y, v);
-  M dot = M(0), a[K];
+  __device__ __forceinline__ void store(const Rows<T>& p, const M (&v)[R][K][DIM]) const {
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      if (!there(q)) break;
+      T* e = p[q];
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < DIM; ++i) e[at(k, i)] = from<T>(v[q][k][i]);
+    }
+  }
+  // steps of R rows, and their codes
+  __device__ __forceinline__ void code(const Rows<signed char>& p, const M (&v)[R][K][DIM], float (&step)[R]) const {
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      unsigned t = 0;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < DIM; ++i) t = max(t, magnitude(v[q][k][i]));
+      float inverse;
+      code_step(__reduce_max_sync(0xffffffffu, t), step[q], inverse);
+      if (!there(q)) continue;
+      signed char* e = p[q];
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < DIM; ++i) e[at(k, i)] = to_code(v[q][k][i], inverse);
+    }
+  }
+  // r of R rows
+  __device__ __forceinline__ void inverse_rms(const M (&v)[R][K][DIM], M inv_n, M eps, M (&r)[R]) const {
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      M part[DIM];
+#pragma unroll
+      for (int i = 0; i < DIM; ++i) part[i] = v[q][0][i] * v[q][0][i];
+#pragma unroll
+      for (int k = 1; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < DIM; ++i) part[i] += v[q][k][i] * v[q][k][i];
+#pragma unroll
+      for (int i = 1; i < DIM; ++i) part[0] += part[i];
+      r[q] = part[0];
+    }
+    warp_sums(r, lane);
+#pragma unroll
+    for (int q = 0; q < R; ++q) r[q] = inverse_sqrt(r[q] * inv_n + eps);
+  }
+};
+
+template <class T, class M, int MODE, bool Q8, int DIM, bool MUL_IR, int K, int R>
+__device__ __forceinline__ void forward_short(const View<M>& c, int left, Rows<T> x, Rows<T> y, Rows<T> g, Rows<signed char> ca, Rows<signed char> cg,
+                                              Rows<signed char> ch, M* stats, int64_t ld_stats) {
+  const Short<T, M, DIM, MUL_IR, K, R> w{c.lane, c.mul, left};
+  M v[R][K][DIM], xv[R][K][DIM], a[R][K], r[R], rh[R];
+  float step[R], gstep[R], hstep[R];
+  w.load((MODE & kBranch) ? y : x, v);
+  if (MODE & kBranch) w.load(x, xv);
+#pragma unroll
+  for (int q = 0; q < R; ++q) {
+    gstep[q] = 0.f;
+    if ((MODE & kBranch) && c.gated) {
+      const T* e = g[w.row(q)];
+      M gate[K];
+#pragma unroll
+      for (int k = 0; k < K; ++k) gate[k] = to<M>(e[c.lane + 32 * k]);
+      if (Q8) {
+        unsigned top = 0;
+        float inverse;
+#pragma unroll
+        for (int k = 0; k < K; ++k) top = max(top, magnitude(gate[k]));
+        code_step(__reduce_max_sync(0xffffffffu, top), gstep[q], inverse);
+        if (w.there(q)) {
+#pragma unroll
+          for (int k = 0; k < K; ++k) cg[q][c.lane + 32 * k] = to_code(gate[k], inverse);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        M de;
+        activation(c.gate, gate[k], a[q][k], de);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k) a[q][k] = M(1);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const M s = ((MODE & kBranch) ? c.s : c.w)[c.lane + 32 * k];
+#pragma unroll
+    for (int q = 0; q < R; ++q) a[q][k] *= s;
+  }
+  w.inverse_rms(v, c.inv_n, c.eps, r);
+  if (Q8) w.code(ca, v, step);
+#pragma unroll
+  for (int q = 0; q < R; ++q)
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < DIM; ++i) v[q][k][i] = (MODE & kBranch) ? xv[q][k][i] + a[q][k] * r[q] * v[q][k][i] : a[q][k] * r[q] * v[q][k][i];
+  w.store(x, v);
+  if (MODE == kBoth) {
+    w.inverse_rms(v, c.inv_n, c.eps, rh);
+    if (Q8) w.code(ch, v, hstep);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const M b = c.w[c.lane + 32 * k];
+#pragma unroll
+      for (int q = 0; q < R; ++q)
+#pragma unroll
+        for (int i = 0; i < DIM; ++i) v[q][k][i] *= b * rh[q];
+    }
+    w.store(y, v);
+  }
+  if (stats && c.lane == 0) {
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      if (!w.there(q)) break;
+      M* e = stats + q * ld_stats;
+      e[0] = r[q];
+      if (MODE == kBoth) e[1] = rh[q];
+      if (Q8) { e[2] = M(step[q]); e[3] = M(gstep[q]); }
+      if (Q8 && MODE == kBoth) e[4] = M(hstep[q]);
+    }
+  }
+}
+
+template <class T, class M, class K8, int MODE, bool Q8, int DIM, bool MUL_IR, int K, int R>
+__device__ __forceinline__ void backward_short(const View<M>& c, int left, Rows<T> go, Rows<T> gn, Rows<K8> h, Rows<K8> y, Rows<K8> g, Rows<T> dg,
+                                               Rows<M> stats, bool has_go) {
+  const Short<T, M, DIM, MUL_IR, K, R> w{c.lane, c.mul, left};
+  M o[R][K][DIM], v[R][K][DIM], dot[R];
+  if (MODE & kNorm) {
+    M rh[R], step[R], p[R][K], b[K];
+    w.load(gn, o);
+    w.load(h, v);
+#pragma unroll
+    for (int k = 0; k < K; ++k) b[k] = c.w[c.lane + 32 * k];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const M* e = stats[w.row(q)];
+      rh[q] = e[MODE == kBoth ? 1 : 0];
+      step[q] = Q8 ? e[MODE == kBoth ? 4 : 2] : M(1);
+      dot[q] = M(0);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        p[q][k] = M(0);
+#pragma unroll
+        for (int i = 0; i < DIM; ++i) p[q][k] += o[q][k][i] * v[q][k][i];
+        p[q][k] *= rh[q] * step[q];
+        dot[q] += b[k] * p[q][k];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      M sum = c.acc_w[c.lane + 32 * k];
+#pragma unroll
+      for (int q = 0; q < R; ++q) sum += w.there(q) ? p[q][k] : M(0);
+      c.acc_w[c.lane + 32 * k] = sum;
+    }
+    warp_sums(dot, c.lane);
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      const M qh = rh[q] * (rh[q] * (c.inv_n * dot[q])) * step[q];
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < DIM; ++i) o[q][k][i] = b[k] * rh[q] * o[q][k][i] - qh * v[q][k][i];
+    }
+    if (MODE == kNorm) {
+      w.store(gn, o);
+      return;
+    }
+    if (has_go) {
+      w.load(go, v);
+#pragma unroll
+      for (int q = 0; q < R; ++q)
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int i = 0; i < DIM; ++i) o[q][k][i] += v[q][k][i];
+    }
+    w.store(go, o);
+  } else {
+    w.load(go, o);
+  }
+  M r[R], step[R], a[R][K];
+  w.load(y, v);
+#pragma unroll
+  for (int q = 0; q < R; ++q) {
+    const M* e = stats[w.row(q)];
+    r[q] = e[0];
+    step[q] = Q8 ? e[2] : M(1);
+    dot[q] = M(0);
+  }
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int u = c.lane + 32 * k;
-    M e = M(1), de = M(0), p = M(0);
-    if (c.gated) activation(c.gate, to<M>(g[u]) * gstep, e, de);
-#pragma unroll
-    for (int i = 0; i < DIM; ++i) p += o[k][i] * v[k][i];
-    p *= r * step;
     const M s = c.s[u];
-    a[k] = s * e;
-    dot += a[k] * p;
-    c.acc_s[u] += e * p;
-    if (c.gated) dg[u] = from<T>(s * de * p);            // may lie over g[u]
+    M sum = c.acc_s[u];
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      M e = M(1), de = M(0), p = M(0);
+      if (c.gated) activation(c.gate, to<M>(g[w.row(q)][u]) * (Q8 ? stats[w.row(q)][3] : M(1)), e, de);
+#pragma unroll
+      for (int i = 0; i < DIM; ++i) p += o[q][k][i] * v[q][k][i];
+      p *= r[q] * step[q];
+      a[q][k] = s * e;
+      dot[q] += a[q][k] * p;
+      sum += w.there(q) ? e * p : M(0);
+      if (c.gated && w.there(q)) dg[q][u] = from<T>(s * de * p);   // may lie over g[q][u], which no later row reads
+    }
+    c.acc_s[u] = sum;
   }
-  const M qy = r * (r * (c.inv_n * cueq::warp_sum(dot))) * step;
+  warp_sums(dot, c.lane);
 #pragma unroll
-  for (int k = 0; k < K; ++k)
+  for (int q = 0; q < R; ++q) {
+    const M qy = r[q] * (r[q] * (c.inv_n * dot[q])) * step[q];
 #pragma unroll
-    for (int i = 0; i < DIM; ++i) v[k][i] = a[k] * r * o[k][i] - qy * v[k][i];
-  q.store(MODE == kBoth ? gn : go, v);
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < DIM; ++i) v[q][k][i] = a[q][k] * r[q] * o[q][k][i] - qy * v[q][k][i];
+  }
+  w.store(MODE == kBoth ? gn : go, v);
 }
 
 // ---- moving rows ----------------------------------------------------------------------------------------------------------
@@ -662,7 +774,7 @@ __device__ __forceinline__ View<M> block_view(const Params& p, const Slice& s, c
   c.mul = b.mul; c.dim = b.dim;
   c.lane = threadIdx.x;
   c.gate = p.gate; c.gated = p.gate != CUEQ_NORM_GATE_NONE;
-  c.inv_n = M(b.inv_n);
+  c.inv_n = reciprocal(M(b.mul * b.dim));
   c.eps = M(p.eps);
   return c;
 }
@@ -678,23 +790,27 @@ __device__ __forceinline__ void put_moves(Move* moves, const Move (&in)[NIN], in
   __syncwarp();
 }
 
-// (dimension, channels per lane) of a block: CALL for those that registers hold, LONG for the others
-#define CUEQ_NORM_K(D, CALL) if (b.mul == 32) CALL(D, 1); else if (b.mul == 64) CALL(D, 2); else if (b.mul == 96) CALL(D, 3); else CALL(D, 4)
-#define CUEQ_NORM_DIMS(CALL, LONG)                                                     \
-  if (b.mul <= 128 && b.mul % 32 == 0 && b.dim <= 7) {                                                    \
+// (dimension, channels per lane) of a block: SHORT for those that registers hold, LONG, row by row, for the others
+#define CUEQ_NORM_K(D, SHORT)                                                          \
+  if (b.mul == 32) { SHORT(D, 1); }                                                    \
+  else if (b.mul == 64) { SHORT(D, 2); }                                               \
+  else if (b.mul == 96) { SHORT(D, 3); }                                               \
+  else { SHORT(D, 4); }
+#define CUEQ_NORM_DIMS(SHORT, LONG)                                                    \
+  if (b.mul <= 128 && b.mul % 32 == 0 && b.dim <= 7) {                                 \
     switch (b.dim) {                                                                   \
-      case 1: CUEQ_NORM_K(1, CALL); break;                                             \
-      case 3: CUEQ_NORM_K(3, CALL); break;                                             \
-      case 5: CUEQ_NORM_K(5, CALL); break;                                             \
-      default: CUEQ_NORM_K(7, CALL); break;                                            \
+      case 1: CUEQ_NORM_K(1, SHORT) break;                                             \
+      case 3: CUEQ_NORM_K(3, SHORT) break;                                             \
+      case 5: CUEQ_NORM_K(5, SHORT) break;                                             \
+      default: CUEQ_NORM_K(7, SHORT) break;                                            \
     }                                                                                  \
   } else {                                                                             \
     switch (b.dim) {                                                                   \
-      case 1: LONG(1); break;                                                          \
-      case 3: LONG(3); break;                                                          \
-      case 5: LONG(5); break;                                                          \
-      case 7: LONG(7); break;                                                          \
-      default: LONG(0); break;                                                         \
+      case 1: LONG(1) break;                                                           \
+      case 3: LONG(3) break;                                                           \
+      case 5: LONG(5) break;                                                           \
+      case 7: LONG(7) break;                                                           \
+      default: LONG(0) break;                                                          \
     }                                                                                  \
   }
 
@@ -727,19 +843,28 @@ __device__ __forceinline__ bool forward_slice(const Params& p, const Slice& sl, 
       const Blk& b = p.blk[k];
       const View<M> c = block_view<M>(p, sl, b, at);
       const int e = b.off - b0.off, u = b.ch - b0.ch;
-      for (int r = 0; r < n; ++r) {
-        M* stats = p.stats ? reinterpret_cast<M*>(p.stats) + ((z + r) * p.nb + k) * p.ns : nullptr;
-        T *px = reinterpret_cast<T*>(s + st.a.at + r * st.a.pitch) + e, *py = reinterpret_cast<T*>(s + st.b.at + r * st.b.pitch) + e;
-        const T* pg = reinterpret_cast<const T*>(s + st.g.at + r * st.g.pitch) + u;
-        signed char *pa = reinterpret_cast<signed char*>(s + st.ca.at + r * st.ca.pitch) + (b.code - b0.code),
-                    *pc = reinterpret_cast<signed char*>(s + st.cg.at + r * st.cg.pitch) + (b.gcode - b0.gcode),
-                    *ph = reinterpret_cast<signed char*>(s + st.ch.at + r * st.ch.pitch) + (b.hcode - b0.hcode);
-#define CUEQ_CALL(D, K) forward_short<T, M, MODE, Q8, D, MUL_IR, K>(c, px, py, pg, pa, pc, ph, stats)
-#define CUEQ_LONG(D) forward_item<T, M, MODE, Q8, D, MUL_IR>(c, px, py, pg, pa, pc, ph, stats)
-        CUEQ_NORM_DIMS(CUEQ_CALL, CUEQ_LONG)
+      auto region = [&](const Region& reg, int bytes) { return s + reg.at + bytes; };
+      const Rows<T> rx{region(st.a, e * size), st.a.pitch}, ry{region(st.b, e * size), st.b.pitch}, rg{region(st.g, u * size), st.g.pitch};
+      const Rows<signed char> ra{region(st.ca, b.code - b0.code), st.ca.pitch}, rc{region(st.cg, b.gcode - b0.gcode), st.cg.pitch},
+          rh{region(st.ch, b.hcode - b0.hcode), st.ch.pitch};
+      const int64_t ld_stats = (int64_t)p.nb * p.ns;
+      M* stats = p.stats ? reinterpret_cast<M*>(p.stats) + z * ld_stats + k * p.ns : nullptr;
+      auto rows_on = [](auto t, int r) { t.base += r * t.pitch; return t; };
+#define CUEQ_ROWS(D, N, R)                                                                                                             \
+  for (int r = 0; r < n; r += R)                                                                                                       \
+    forward_short<T, M, MODE, Q8, D, MUL_IR, N, R>(c, n - r, rows_on(rx, r), rows_on(ry, r), rows_on(rg, r), rows_on(ra, r), rows_on(rc, r), \
+                                                   rows_on(rh, r), stats ? stats + r * ld_stats : nullptr, ld_stats);
+#define CUEQ_SHORT(D, N)                                                                                                               \
+  if constexpr (kRowsAtOnce<D, N> > 1) {                                                                                               \
+    if (n > 1) { CUEQ_ROWS(D, N, (kRowsAtOnce<D, N>)) } else { CUEQ_ROWS(D, N, 1) }                                                    \
+  } else { CUEQ_ROWS(D, N, 1) }
+#define CUEQ_LONG(D)                                                                                                                   \
+  for (int r = 0; r < n; ++r)                                                                                                          \
+    forward_item<T, M, MODE, Q8, D, MUL_IR>(c, rx[r], ry[r], rg[r], ra[r], rc[r], rh[r], stats ? stats + r * ld_stats : nullptr);
+      CUEQ_NORM_DIMS(CUEQ_SHORT, CUEQ_LONG)
 #undef CUEQ_LONG
-#undef CUEQ_CALL
-      }
+#undef CUEQ_SHORT
+#undef CUEQ_ROWS
     }
   });
 }
@@ -783,18 +908,26 @@ __device__ __forceinline__ bool backward_slice(const Params& p, const Slice& sl,
       const View<M> c = block_view<M>(p, sl, b, at);
       const int e = b.off - b0.off, u = b.ch - b0.ch;
       const int ce = Q8 ? b.code - b0.code : e, he = Q8 ? (MODE == kBoth ? b.hcode - b0.hcode : b.code - b0.code) : e, ge = Q8 ? b.gcode - b0.gcode : u;
-      for (int r = 0; r < n; ++r) {
-        T *pa = reinterpret_cast<T*>(s + st.a.at + r * st.a.pitch) + e, *pb = reinterpret_cast<T*>(s + st.b.at + r * st.b.pitch) + e;
-        const K *ph = reinterpret_cast<const K*>(s + st.c.at + r * st.c.pitch) + he, *py = reinterpret_cast<const K*>(s + st.d.at + r * st.d.pitch) + ce,
-                *pg = reinterpret_cast<const K*>(s + st.g.at + r * st.g.pitch) + ge;
-        T* pd = reinterpret_cast<T*>(s + st.dg.at + r * st.dg.pitch) + u;
-        const M* ps = reinterpret_cast<const M*>(s + st.st.at + r * st.st.pitch) + (k - sl.first) * p.ns;
-#define CUEQ_CALL(D, N) backward_short<T, M, K, MODE, Q8, D, MUL_IR, N>(c, pa, pb, ph, py, pg, pd, ps, has_go)
-#define CUEQ_LONG(D) backward_item<T, M, K, MODE, Q8, D, MUL_IR>(c, pa, pb, ph, py, pg, pd, ps, has_go)
-        CUEQ_NORM_DIMS(CUEQ_CALL, CUEQ_LONG)
+      auto region = [&](const Region& reg, int bytes) { return s + reg.at + bytes; };
+      const Rows<T> ra{region(st.a, e * size), st.a.pitch}, rb{region(st.b, e * size), st.b.pitch}, rd{region(st.dg, u * size), st.dg.pitch};
+      const Rows<K> rh{region(st.c, he * (int)sizeof(K)), st.c.pitch}, ry{region(st.d, ce * (int)sizeof(K)), st.d.pitch},
+          rg{region(st.g, ge * (int)sizeof(K)), st.g.pitch};
+      const Rows<M> rs{region(st.st, (k - sl.first) * stat), st.st.pitch};
+      auto rows_on = [](auto t, int r) { t.base += r * t.pitch; return t; };
+#define CUEQ_ROWS(D, N, R)                                                                                                             \
+  for (int r = 0; r < n; r += R)                                                                                                       \
+    backward_short<T, M, K, MODE, Q8, D, MUL_IR, N, R>(c, n - r, rows_on(ra, r), rows_on(rb, r), rows_on(rh, r), rows_on(ry, r), rows_on(rg, r), \
+                                                       rows_on(rd, r), rows_on(rs, r), has_go);
+#define CUEQ_SHORT(D, N)                                                                                                               \
+  if constexpr (kRowsAtOnce<D, N> > 1) {                                                                                               \
+    if (n > 1) { CUEQ_ROWS(D, N, (kRowsAtOnce<D, N>)) } else { CUEQ_ROWS(D, N, 1) }                                                    \
+  } else { CUEQ_ROWS(D, N, 1) }
+#define CUEQ_LONG(D)                                                                                                                   \
+  for (int r = 0; r < n; ++r) backward_item<T, M, K, MODE, Q8, D, MUL_IR>(c, ra[r], rb[r], rh[r], ry[r], rg[r], rd[r], rs[r], has_go);
+      CUEQ_NORM_DIMS(CUEQ_SHORT, CUEQ_LONG)
 #undef CUEQ_LONG
-#undef CUEQ_CALL
-      }
+#undef CUEQ_SHORT
+#undef CUEQ_ROWS
     }
   });
   // this warp's sums of the parameters' gradients

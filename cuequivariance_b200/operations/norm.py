@@ -21,6 +21,7 @@ from ..executor import dtype_code
 from ..irreps import Irreps, IrrepsLayout
 
 SAVED_ACTIVATIONS = ("full", "int8")
+_TYPES = (torch.float32, torch.float64, torch.bfloat16, torch.float16)
 
 
 def check_saved_activations(value: str) -> bool:
@@ -32,7 +33,7 @@ def check_saved_activations(value: str) -> bool:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` with unit stride along the row and rows that do not overlap (or are all the same one)."""
-    if (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.stride(0) == 0 or t.shape[0] <= 1):
+    if t.is_contiguous() or (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.stride(0) == 0 or t.shape[0] <= 1):
         return t
     return t.contiguous()
 
@@ -52,11 +53,12 @@ class _Block:
         pad = lambda n: (n + 15) // 16 * 16  # noqa: E731
         features = sum(pad(m * d) for m, d in muls)
         self.code_bytes = features * (2 if mode == _lib.NORM_BOTH else 1) + (sum(pad(m) for m, _ in muls) if gate else 0)
+        self._arguments = {}
         self.stats_stride = 8 if int8 and mode == _lib.NORM_BOTH else 4
 
     def __getstate__(self):
         state = dict(self.__dict__)
-        state["blocks"] = [(b.mul, b.dim) for b in self.blocks]
+        state["blocks"], state["_arguments"] = [(b.mul, b.dim) for b in self.blocks], {}
         return state
 
     def __setstate__(self, state):
@@ -64,17 +66,18 @@ class _Block:
         self.blocks = (_lib.NormBlock * len(state["blocks"]))(*state["blocks"])
 
     def check(self, name: str, t: torch.Tensor, width: int, like: Optional[torch.Tensor] = None) -> None:
-        if t.dim() != 2 or t.shape[1] != width:
-            raise ValueError(f"{name} must have shape (batch, {width}), got {tuple(t.shape)}")
+        shape = t.shape
+        if len(shape) != 2 or shape[1] != width:
+            raise ValueError(f"{name} must have shape (batch, {width}), got {tuple(shape)}")
         if not t.is_cuda:
             raise RuntimeError("cuequivariance_b200 executes on CUDA devices only (there is no CPU fallback)")
-        if like is not None and (t.shape[0] != like.shape[0] or t.dtype != like.dtype or t.device != like.device):
-            raise ValueError(f"{name} must have the rows, dtype and device of x: {tuple(t.shape)} {t.dtype} {t.device} "
+        if like is not None and (shape[0] != like.shape[0] or t.dtype != like.dtype or t.device != like.device):
+            raise ValueError(f"{name} must have the rows, dtype and device of x: {tuple(shape)} {t.dtype} {t.device} "
                              f"against {tuple(like.shape)} {like.dtype} {like.device}")
 
     def check_x(self, x: torch.Tensor) -> None:
         self.check("x", x, self.dim)
-        if x.dtype not in (torch.float32, torch.float64, torch.bfloat16, torch.float16):
+        if x.dtype not in _TYPES:
             raise ValueError(f"unsupported dtype {x.dtype}")
         if self.int8 and x.dtype == torch.float64:
             raise ValueError("saved_activations='int8' is for float32, bfloat16 and float16; float64 activations are kept in full")
@@ -84,23 +87,36 @@ class _Block:
             raise ValueError(f"{name} should not be None")
         if t.shape != (self.channels,) or t.device != x.device:
             raise ValueError(f"{name} must have shape ({self.channels},) on {x.device}, got {tuple(t.shape)} on {t.device}")
-        if t.dtype not in (torch.float32, torch.float64, torch.bfloat16, torch.float16) or (x.dtype == torch.float64) != (t.dtype == torch.float64):
+        if t.dtype not in _TYPES or (x.dtype == torch.float64) != (t.dtype == torch.float64):
             raise ValueError(f"{name} has dtype {t.dtype}, features {x.dtype}: float64 goes with float64 only")
 
     def arguments(self, mode: int, x: torch.Tensor, parameter: torch.Tensor) -> "_lib.NormArgs":
-        a = _lib.NormArgs()
-        a.struct_bytes, a.mode, a.gate, a.mul_ir = C.sizeof(a), mode, _lib.NORM_GATES[self.gate], int(self.layout is IrrepsLayout.mul_ir)
-        a.dtype, a.param_dtype, a.num_blocks, a.stats_stride = dtype_code(x.dtype), dtype_code(parameter.dtype), len(self.blocks), self.stats_stride
-        a.blocks, a.rows, a.eps = self.blocks, x.shape[0], self.eps
-        a.status = _lib.status_word(x.device).data_ptr()
+        """The argument block of a call, without pointers to tensors; what does not change from call to call is kept per type."""
+        key = (mode, x.dtype, parameter.dtype, x.device)
+        kept = self._arguments.get(key)
+        if kept is None:
+            a = _lib.NormArgs()
+            a.struct_bytes, a.mode, a.gate, a.mul_ir = C.sizeof(a), mode, _lib.NORM_GATES[self.gate], int(self.layout is IrrepsLayout.mul_ir)
+            a.dtype, a.param_dtype, a.num_blocks, a.stats_stride = dtype_code(x.dtype), dtype_code(parameter.dtype), len(self.blocks), self.stats_stride
+            a.blocks, a.eps = self.blocks, self.eps
+            a.status = _lib.status_word(x.device).data_ptr()
+            kept = self._arguments[key] = bytes(a)
+        a = _lib.NormArgs.from_buffer_copy(kept)
+        a.rows = x.shape[0]
         return a
 
     def launch(self, which: str, a: "_lib.NormArgs", device: torch.device) -> None:
         L = _lib.lib()
-        name = {_lib.NORM_BRANCH: "gated_residual", _lib.NORM_ALONE: "irreps_norm", _lib.NORM_BOTH: "gated_residual_norm"}[a.mode]
-        with _lib.on_device(device), profiling.kernel(f"{name}_{which}"):
-            fn = L.cueq_b200_norm_forward if which == "forward" else L.cueq_b200_norm_backward
-            _lib.check(fn(C.byref(a), C.c_void_p(torch.cuda.current_stream(device).cuda_stream)))
+        fn = L.cueq_b200_norm_forward if which == "forward" else L.cueq_b200_norm_backward
+        with _lib.on_device(device):
+            stream = torch._C._cuda_getCurrentRawStream(device.index)
+            if not profiling.enabled():
+                profiling.launch_count += 1
+                _lib.check(fn(C.byref(a), stream))
+                return
+            name = {_lib.NORM_BRANCH: "gated_residual", _lib.NORM_ALONE: "irreps_norm", _lib.NORM_BOTH: "gated_residual_norm"}[a.mode]
+            with profiling.kernel(f"{name}_{which}"):
+                _lib.check(fn(C.byref(a), stream))
 
     def forward(self, keep: bool, x, y, g, s, w):
         """(out, norm, codes, stats) - the last two for a backward pass to come."""
@@ -165,8 +181,8 @@ class _Block:
         if codes is not None:
             a.codes, a.ld_codes = codes.data_ptr(), self.code_bytes
         if rows:
-            n = _lib.lib().cueq_b200_norm_parts(C.byref(a))
-            parts = torch.empty(max(n, 0), dtype=stats.dtype, device=like.device)
+            n = max(_lib.lib().cueq_b200_norm_parts(C.byref(a)), 0)
+            parts = torch.empty(n, dtype=stats.dtype, device=like.device)
             a.parts, a.parts_values = parts.data_ptr(), n
             self.launch("backward", a, like.device)
         else:
@@ -190,16 +206,23 @@ class _Norm(torch.autograd.Function):
         return tuple(t for t in (out, norm) if t is not None)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
-        block = ctx.block
-        go = grads[0] if block.mode & _lib.NORM_BRANCH else None
-        gn = grads[-1] if block.mode & _lib.NORM_ALONE else None
-        if go is None and gn is None:
-            return (None,) * 6
-        y, g, h, codes, stats, s, w = ctx.saved_tensors
-        grads = block.backward(go, gn, y, g, h, codes, stats, s, w)
-        return (None, *(t if need else None for t, need in zip(grads, ctx.needs_input_grad[1:])))
+        # once_differentiable is there for the error on a second derivative; it costs 4 us a call
+        return _gradients_once(ctx, *grads) if torch.is_grad_enabled() else _gradients(ctx, *grads)
+
+
+def _gradients(ctx, *grads):
+    block = ctx.block
+    go = grads[0] if block.mode & _lib.NORM_BRANCH else None
+    gn = grads[-1] if block.mode & _lib.NORM_ALONE else None
+    if go is None and gn is None:
+        return (None,) * 6
+    y, g, h, codes, stats, s, w = ctx.saved_tensors
+    grads = block.backward(go, gn, y, g, h, codes, stats, s, w)
+    return (None, *(t if need else None for t, need in zip(grads, ctx.needs_input_grad[1:])))
+
+
+_gradients_once = torch.autograd.function.once_differentiable(_gradients)
 
 
 def _run(block: _Block, x, y, g, s, w):

@@ -84,7 +84,7 @@ def _residual(irreps, rows, dtype, layout, gate, norm_output, saved="full", seed
 SHAPES = [
     (L3, 1), (L3, 37), (L3, 2003),
     ("1x0e", 5), ("1x0e+1x1o+1x2e", 9), ("5x0e+3x1o+2x2e", 301), ("33x0e+7x1o", 64),
-    ("32x0e+32x1o+32x2e+32x3o", 1511), ("64x0e+64x1o", 4099), ("96x0o+48x1e+16x2e+4x4e", 333),
+    ("32x0e+32x1o+32x2e+32x3o", 1511), ("64x0e+64x1o", 4099), ("64x0e+32x0o+32x1o", 6), ("96x0e+64x2e+32x3o", 131), ("129x0e+97x1o", 47), ("96x0o+48x1e+16x2e+4x4e", 333),
     ("300x0e+260x3o", 55), ("2048x0e", 70), ("16x0e+16x0o+16x1e+16x1o+8x5o", 129),
 ]
 
@@ -221,6 +221,15 @@ def test_gradients_against_differences():
                 down = value([t - 1e-6 * direction if q == k else t for q, t in enumerate(d)])
             got = (grads[k] * direction).sum()
             assert abs((up - down) / 2e-6 - got) <= 1e-6 * (1 + abs(got)), names[k]
+
+
+def test_second_derivatives_are_refused():
+    m = cb.GatedResidual("32x0e+3x1o", norm_output=True).to(DEV)
+    x, g = torch.randn(5, 41, device=DEV, requires_grad=True), torch.randn(5, 35, device=DEV)
+    out, n = m(x, x, g)
+    (gx,) = torch.autograd.grad(out.sum() + n.pow(2).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        gx.sum().backward()
 
 
 def test_no_rows():
