@@ -410,11 +410,17 @@ __global__ void __launch_bounds__(kMapThreads, 1) linear_map_kernel(const __grid
 // cp.async instead: 460 us against 315 us.
 constexpr int kGwWorkers = 512;
 constexpr int kGwThreads = 224 + kGwWorkers;
-constexpr int kGwOps = 0;                                  // 2 stages x (x hi, x lo, g hi, g lo)
-constexpr int kGwRawStages = 3;
-constexpr int kGwRaw = 2 * 4 * kBlk;                       // raw rows: x part [16 KiB], g part [16 KiB] per stage
-constexpr int kGwBars = kGwRaw + kGwRawStages * 2 * kBlk;
-constexpr size_t kGwSmem = kGwBars + 128 + 1024;
+// Shared memory: operand stages (x hi, x lo unless x is in codes, g hi, g lo), then stages of raw rows (x part, g part).  With x in codes
+// there is room for one more of each, and the workers take blocks in turn in two groups: what a block waits for between its
+// barriers then overlaps with the other group's block.
+template <bool CODES>
+struct Gw {
+  static constexpr int kGroups = CODES ? 2 : 1;
+  static constexpr int kOpStages = CODES ? 3 : 2, kG = CODES ? kBlk : 2 * kBlk, kOpBytes = kG + 2 * kBlk;
+  static constexpr int kRawStages = CODES ? 4 : 3, kSteps = 4096, kRawG = CODES ? kSteps + 256 : kBlk, kRawBytes = kRawG + kBlk;
+  static constexpr int kRaw = kOpStages * kOpBytes, kBars = kRaw + kRawStages * kRawBytes;   // steps: behind 4 KiB of codes at most, 40 at most
+  static constexpr size_t kSmem = kBars + 160 + 1024;
+};
 
 // raw rows of the block's nodes -> K-major split tile; thread = (channel, quarter of the k range).  Reads are free of bank
 // conflicts: neighbouring channels are d (odd) or 1 floats apart.
@@ -444,14 +450,13 @@ __device__ __forceinline__ void gw_transpose(const float* raw, unsigned char* hi
   }
 }
 
-// x in 8 bits -> K-major tile: a code is exact, so there is no lo half
-template <int D, bool MUL_IR>
-__device__ __forceinline__ void gw_transpose_codes(const signed char* raw, unsigned char* hi, int C, int nodes, int tid) {
-  const int ch = tid & 127;
-  if (ch >= C) return;
+// x in 8 bits -> K-major tile (a code is exact, so there is no lo half), and g rows times the steps of their nodes -> K-major split
+// tile; thread = (channel, half of the k range)
+template <int D, bool MUL_IR, int HALF>
+__device__ __forceinline__ void gw_codes_half(const signed char* raw, unsigned char* hi, int ch, int C, int nodes) {
 #pragma unroll
-  for (int gg = 0; gg < 2; ++gg) {
-    const int chunk = (tid >> 7) * 2 + gg;
+  for (int gg = 0; gg < 4; ++gg) {
+    const int chunk = HALF * 4 + gg;
     float v[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -461,14 +466,11 @@ __device__ __forceinline__ void gw_transpose_codes(const signed char* raw, unsig
     *reinterpret_cast<float4*>(hi + ch * 128 + ((chunk ^ (ch & 7)) << 4)) = make_float4(v[0], v[1], v[2], v[3]);
   }
 }
-// g rows times the steps of their nodes -> K-major split tile
-template <int D, bool MUL_IR>
-__device__ __forceinline__ void gw_transpose_steps(const float* raw, unsigned char* hi, int C, int nodes, int tid, const float* steps) {
-  const int ch = tid & 127;
-  if (ch >= C) return;
+template <int D, bool MUL_IR, int HALF>
+__device__ __forceinline__ void gw_steps_half(const float* raw, unsigned char* hi, int ch, int C, int nodes, const float* steps) {
 #pragma unroll
-  for (int gg = 0; gg < 2; ++gg) {
-    const int chunk = (tid >> 7) * 2 + gg;
+  for (int gg = 0; gg < 4; ++gg) {
+    const int chunk = HALF * 4 + gg;
     float v[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -478,23 +480,37 @@ __device__ __forceinline__ void gw_transpose_steps(const float* raw, unsigned ch
     store_split(hi, hi + kBlk, ch, chunk, v);
   }
 }
-constexpr int kGwSteps = kBlk - 256;     // the steps of a block's nodes, behind the codes: 4 KiB of codes at most, 40 steps at most
+template <int D, bool MUL_IR>
+__device__ __forceinline__ void gw_codes(const signed char* raw, unsigned char* hi, int C, int nodes, int tid) {
+  const int ch = tid & 127;
+  if (ch >= C) return;
+  if (tid < 128) gw_codes_half<D, MUL_IR, 0>(raw, hi, ch, C, nodes);
+  else gw_codes_half<D, MUL_IR, 1>(raw, hi, ch, C, nodes);
+}
+template <int D, bool MUL_IR>
+__device__ __forceinline__ void gw_steps(const float* raw, unsigned char* hi, int C, int nodes, int tid, const float* steps) {
+  const int ch = tid & 127;
+  if (ch >= C) return;
+  if (tid < 128) gw_steps_half<D, MUL_IR, 0>(raw, hi, ch, C, nodes, steps);
+  else gw_steps_half<D, MUL_IR, 1>(raw, hi, ch, C, nodes, steps);
+}
 
 template <bool CODES>
 __global__ void __launch_bounds__(kGwThreads, 1) linear_gw_kernel(const __grid_constant__ LParams p) {
+  using G = Gw<CODES>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  unsigned long long* rawfull = reinterpret_cast<unsigned long long*>(base + kGwBars);
-  unsigned long long* rawempty = rawfull + kGwRawStages;
-  unsigned long long* opfull = rawempty + kGwRawStages;
-  unsigned long long* opempty = opfull + 2;
-  unsigned long long* accfull = opempty + 2;
+  unsigned long long* rawfull = reinterpret_cast<unsigned long long*>(base + G::kBars);
+  unsigned long long* rawempty = rawfull + G::kRawStages;
+  unsigned long long* opfull = rawempty + G::kRawStages;
+  unsigned long long* opempty = opfull + G::kOpStages;
+  unsigned long long* accfull = opempty + G::kOpStages;
   unsigned long long* accempty = accfull + 1;
   unsigned* tmem_slot = reinterpret_cast<unsigned*>(accempty + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kGwRawStages; ++s) { bar_init(rawfull + s, 2); bar_init(rawempty + s, kGwWorkers / 32); }
-    for (int s = 0; s < 2; ++s) { bar_init(opfull + s, kGwWorkers / 32); bar_init(opempty + s, 1); }
+    for (int s = 0; s < G::kRawStages; ++s) { bar_init(rawfull + s, 2); bar_init(rawempty + s, kGwWorkers / 32 / G::kGroups); }
+    for (int s = 0; s < G::kOpStages; ++s) { bar_init(opfull + s, kGwWorkers / 32 / G::kGroups); bar_init(opempty + s, 1); }
     bar_init(accfull, 1);
     bar_init(accempty, 4);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -541,14 +557,14 @@ __global__ void __launch_bounds__(kGwThreads, 1) linear_gw_kernel(const __grid_c
         ok = ok && bar_wait(accempty, (run & 1) ^ 1, p.status);
         ++run;
         for (int b = 0; b < blocks && ok; ++b, ++it) {
-          const unsigned s = it & 1;
-          ok = bar_wait(opfull + s, (it >> 1) & 1, p.status);
+          const unsigned s = it % G::kOpStages;
+          ok = bar_wait(opfull + s, (it / G::kOpStages) & 1, p.status);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-          const unsigned char* st = base + kGwOps + s * 4 * kBlk;
-          if (!CODES) umma_block(tmem_base + 3 * 128, st + kBlk, st + 2 * kBlk, idesc, b ? 1u : 0u);
-          umma_block(tmem_base + 3 * 128, st, st + 3 * kBlk, idesc, !CODES || b ? 1u : 0u);
-          umma_block(tmem_base + (b % 3) * 128, st, st + 2 * kBlk, idesc, b >= 3 ? 1u : 0u);
+          const unsigned char* st = base + s * G::kOpBytes;
+          if (!CODES) umma_block(tmem_base + 3 * 128, st + kBlk, st + G::kG, idesc, b ? 1u : 0u);
+          umma_block(tmem_base + 3 * 128, st, st + G::kG + kBlk, idesc, !CODES || b ? 1u : 0u);
+          umma_block(tmem_base + (b % 3) * 128, st, st + G::kG, idesc, b >= 3 ? 1u : 0u);
           umma_commit(opempty + s);
         }
         if (ok) umma_commit(accfull);
@@ -567,45 +583,48 @@ __global__ void __launch_bounds__(kGwThreads, 1) linear_gw_kernel(const __grid_c
                                         : (const unsigned char*)(is_g ? p.g + q.o_off : p.x + q.x_off)) + (int64_t)z0 * ld;
       const float* steps = codes ? p.steps + (&q - p.path) * p.ld_steps : nullptr;
       for (int b = 0; b < blocks && ok; ++b, ++it, src += n * ld) {
-        const unsigned s = it % kGwRawStages;
-        ok = bar_wait(rawempty + s, ((it / kGwRawStages) & 1) ^ 1, p.status);
+        const unsigned s = it % G::kRawStages;
+        ok = bar_wait(rawempty + s, ((it / G::kRawStages) & 1) ^ 1, p.status);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const int nodes = min(n, zend - (z0 + b * n));
-        const unsigned raw = s32(base + kGwRaw + s * 2 * kBlk + (is_g ? kBlk : 0));
+        const unsigned raw = s32(base + G::kRaw + s * G::kRawBytes + (is_g ? G::kRawG : 0));
         // steps: whole groups of four, the first and the last may hold other nodes' as well
         const int s0 = (z0 + b * n) & ~3, s1 = (z0 + b * n + nodes + 3) & ~3;
         if (lane == 0) bar_expect_tx(rawfull + s, nodes * bytes + (codes ? (s1 - s0) * 4 : 0));
         __syncwarp();
         if (codes && lane == 0)
           asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
-                       ::"r"(raw + kGwSteps), "l"(steps + s0), "r"((s1 - s0) * 4), "r"(s32(rawfull + s)) : "memory");
+                       ::"r"(raw + G::kSteps), "l"(steps + s0), "r"((s1 - s0) * 4), "r"(s32(rawfull + s)) : "memory");
         if (lane < nodes)                                            // one node per lane; at most 32 / d of them
           asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
                        ::"r"(raw + lane * bytes), "l"(src + lane * ld), "r"(bytes), "r"(s32(rawfull + s)) : "memory");
       }
     });
   } else {
-    const int tid = threadIdx.x - 160;
+    constexpr int kGroup = kGwWorkers / G::kGroups;
+    const int group = (threadIdx.x - 160) / kGroup, tid = (threadIdx.x - 160) % kGroup;
     unsigned it = 0;
     bool dead = false;
     for_each_run(p, first, last, rows_per_block, [&](const LPath& q, int, int z0, int zend, int blocks) {
       const int n = rows_per_block(q.d);
       for (int b = 0; b < blocks; ++b, ++it) {
-        const unsigned r = it % kGwRawStages, s = it & 1;
-        if (!dead) dead = !bar_wait(rawfull + r, (it / kGwRawStages) & 1, p.status);
-        if (!dead) dead = !bar_wait(opempty + s, ((it >> 1) & 1) ^ 1, p.status);
-        const float* raw = reinterpret_cast<const float*>(base + kGwRaw + r * 2 * kBlk);
-        unsigned char* st = base + kGwOps + s * 4 * kBlk;
+        if (G::kGroups > 1 && (int)(it % G::kGroups) != group) continue;
+        const unsigned r = it % G::kRawStages, s = it % G::kOpStages;
+        if (!dead) dead = !bar_wait(rawfull + r, (it / G::kRawStages) & 1, p.status);
+        if (!dead) dead = !bar_wait(opempty + s, ((it / G::kOpStages) & 1) ^ 1, p.status);
+        const unsigned char* raw = base + G::kRaw + r * G::kRawBytes;
+        const float* raw_g = reinterpret_cast<const float*>(raw + G::kRawG);
+        unsigned char* st = base + s * G::kOpBytes;
         const int nodes = min(n, zend - (z0 + b * n));
         if (!dead) {
           if (CODES) {
-            const float* steps = raw + kGwSteps / 4 + ((z0 + b * n) & 3);
-            LINEAR_DISPATCH(gw_transpose_codes, q.d, p.x_mul_ir, reinterpret_cast<const signed char*>(raw), st, q.K, nodes, tid)
-            LINEAR_DISPATCH(gw_transpose_steps, q.d, p.o_mul_ir, raw + kBlk / 4, st + 2 * kBlk, q.N, nodes, tid, steps)
+            const float* steps = reinterpret_cast<const float*>(raw + G::kSteps) + ((z0 + b * n) & 3);
+            LINEAR_DISPATCH(gw_codes, q.d, p.x_mul_ir, reinterpret_cast<const signed char*>(raw), st, q.K, nodes, tid)
+            LINEAR_DISPATCH(gw_steps, q.d, p.o_mul_ir, raw_g, st + G::kG, q.N, nodes, tid, steps)
           } else {
-            LINEAR_DISPATCH(gw_transpose, q.d, p.x_mul_ir, raw, st, q.K, nodes, tid)
-            LINEAR_DISPATCH(gw_transpose, q.d, p.o_mul_ir, raw + kBlk / 4, st + 2 * kBlk, q.N, nodes, tid)
+            LINEAR_DISPATCH(gw_transpose, q.d, p.x_mul_ir, reinterpret_cast<const float*>(raw), st, q.K, nodes, tid)
+            LINEAR_DISPATCH(gw_transpose, q.d, p.o_mul_ir, raw_g, st + G::kG, q.N, nodes, tid)
           }
         }
         publish(opfull + s, lane);
@@ -831,11 +850,12 @@ int launch_gw(const cueq_linear_args* a, const cueq_linear_codes* codes, void* s
   }
   static cueq::PerDeviceFlag configured[2];
   const auto kernel = codes ? linear_gw_kernel<true> : linear_gw_kernel<false>;
+  const size_t smem = codes ? Gw<true>::kSmem : Gw<false>::kSmem;
   if (!configured[codes != nullptr].get()) {
-    CUEQ_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGwSmem));
+    CUEQ_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     configured[codes != nullptr].set();
   }
-  kernel<<<grid, kGwThreads, kGwSmem, reinterpret_cast<cudaStream_t>(stream)>>>(p);
+  kernel<<<grid, kGwThreads, smem, reinterpret_cast<cudaStream_t>(stream)>>>(p);
   CUEQ_CUDA_OK(cudaGetLastError());
   linear_gw_sum_kernel<<<dim3((widest / 4 + 127) / 128, p.num_paths * p.num_classes), 128, 0, reinterpret_cast<cudaStream_t>(stream)>>>(p, t, grid);
   CUEQ_CUDA_OK(cudaGetLastError());
