@@ -12,7 +12,7 @@
 // What bounds them: the rows are read once and written once, 2 * 268 MB each for 32,768 nodes of 128x(0e+1o+2e+3o);
 // 82 us at 6.5 TB/s against 46 us of three-pass TF32.  The layer used to be one GEMM launch per irrep and component
 // (48 of them, the row reductions on 32 thread blocks), with layout transpositions around them and the weights split by
-// elementwise kernels: 3.25 ms for forward and both gradients.  Now 0.62 ms: linear_map 195 us (2.75 TB/s), linear_gw 212 us.
+// elementwise kernels: 3.25 ms for forward and both gradients.  Now 0.62 ms: linear_map 195 us (2.75 TB/s), linear_gw 212 us, with x in codes 153 us (and 58 us to write them).
 // What is left is the latency between load, split and MMA: tensor pipe 23 % and HBM 45 % busy.
 //
 // The components of an irrep share its weight block, so rows (z, i) are folded into the M axis of the MMA (linear_map)
@@ -56,6 +56,7 @@ struct LParams {
   int64_t ldx, ldo, w_class_stride;
   int x_mul_ir, o_mul_ir, num_paths, num_classes;
   int total;            // tiles (linear_map) or K blocks (linear_gw) over all paths and classes
+  int64_t total_cost;   // linear_gw: of all K blocks
   int* status;
   LPath path[kMaxPaths];
   int bounds[kMaxClasses + 1];
@@ -63,6 +64,11 @@ struct LParams {
 
 __host__ __device__ constexpr int rows_per_tile(int d) { return 128 / d; }     // nodes per tile of linear_map
 __host__ __device__ constexpr int rows_per_block(int d) { return 32 / d; }     // nodes per K block of linear_gw
+
+// Cost of a K block of linear_gw, in which the thread blocks' shares are equal.  With x in codes a block of 32 scalars, 64 short bulk copies, takes
+// 1.45 times as long as one of vectors (214 against 148 us for 17,760 blocks); dealt out by number, the thread blocks with scalars kept the
+// others waiting for a third of the time.  With x as it is the ratio is 1.16 and numbers are equal.
+template <bool CODES> __host__ __device__ constexpr int gw_cost(int d) { return !CODES ? 1 : d == 1 ? 3 : 2; }
 
 // The runs of consecutive items (tiles / K blocks) of one path and class that fall into [first, last): calls
 // f(path, class, z of the run's first item, z end of the class, items).  Every role of a thread block walks the same runs.
@@ -495,6 +501,21 @@ __device__ __forceinline__ void gw_steps(const float* raw, unsigned char* hi, in
   else gw_steps_half<D, MUL_IR, 1>(raw, hi, ch, C, nodes, steps);
 }
 
+// the K block in which the cost of all blocks before reaches `cost`
+template <bool CODES>
+__device__ __forceinline__ int gw_item(const LParams& p, int64_t cost) {
+  int start = 0;
+  for (int q = 0; q < p.num_paths; ++q) {
+    const int n = rows_per_block(p.path[q].d), w = gw_cost<CODES>(p.path[q].d);
+    int items = 0;
+    for (int c = 0; c < p.num_classes; ++c) items += (p.bounds[c + 1] - p.bounds[c] + n - 1) / n;
+    if (cost < (int64_t)items * w) return start + (int)(cost / w);
+    cost -= (int64_t)items * w;
+    start += items;
+  }
+  return start;
+}
+
 template <bool CODES>
 __global__ void __launch_bounds__(kGwThreads, 1) linear_gw_kernel(const __grid_constant__ LParams p) {
   using G = Gw<CODES>;
@@ -516,7 +537,7 @@ __global__ void __launch_bounds__(kGwThreads, 1) linear_gw_kernel(const __grid_c
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   const unsigned tmem_base = tmem_alloc_all(tmem_slot, warp, 4);
-  const int first = (int)((int64_t)p.total * blockIdx.x / gridDim.x), last = (int)((int64_t)p.total * (blockIdx.x + 1) / gridDim.x);
+  const int first = gw_item<CODES>(p, p.total_cost * blockIdx.x / gridDim.x), last = gw_item<CODES>(p, p.total_cost * (blockIdx.x + 1) / gridDim.x);
 
   if (warp < 4) {
     unsigned run = 0;
@@ -637,16 +658,16 @@ __global__ void __launch_bounds__(kGwThreads, 1) linear_gw_kernel(const __grid_c
 
 // The runs of one (path, class) added up in their order and put into the gradient.  Before, every run was added to the
 // gradient by red.global.add, and the last bits changed from call to call.
-// start[s]: first K block of (path, class) s = path * num_classes + class; the thread block of a K block t is the largest b
-// with total * b / blocks <= t.
-struct GwStarts { int start[kMaxPaths * kMaxClasses + 1]; };
+// start[s]: cost of the K blocks before (path, class) s = path * num_classes + class.  The thread block of a K block is the largest b whose first
+// cost, total_cost * b / blocks, lies before the block's end.
+struct GwStarts { int64_t start[kMaxPaths * kMaxClasses + 1]; int cost[kMaxPaths]; };
 __global__ void __launch_bounds__(128) linear_gw_sum_kernel(const __grid_constant__ LParams p, const __grid_constant__ GwStarts t, int blocks) {
   const int s = blockIdx.y, cls = s % p.num_classes;
   const LPath& q = p.path[s / p.num_classes];
   const int e = (blockIdx.x * 128 + threadIdx.x) * 4;
   if (e >= q.K * q.N || !status_clean(p.status)) return;
-  auto block_of = [&](int64_t item) { return (int)(((item + 1) * blocks + p.total - 1) / p.total) - 1; };
-  const int b0 = block_of(t.start[s]), n = t.start[s] == t.start[s + 1] ? 0 : block_of(t.start[s + 1] - 1) - b0 + 1;   // 0: a class without rows
+  auto block_of = [&](int64_t end) { return (int)((end * blocks + p.total_cost - 1) / p.total_cost) - 1; };
+  const int b0 = block_of(t.start[s] + t.cost[s / p.num_classes]), n = t.start[s] == t.start[s + 1] ? 0 : block_of(t.start[s + 1]) - b0 + 1;   // 0: a class without rows
   const float* src = p.parts + (int64_t)(b0 + s) * p.slot + e;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
@@ -699,11 +720,29 @@ int make_params(const cueq_linear_args* a, PerItem per_item, bool gw, LParams* p
 
 // every run ends with 64 KB of partial sums, so short inputs use fewer blocks; long ones are cut so that an accumulation
 // chain does not grow with the number of rows
+template <bool CODES>
 int gw_blocks(const LParams& p) {
+  int unit = gw_cost<CODES>(p.path[0].d);      // of the cheapest block
+  for (int k = 1; k < p.num_paths; ++k) unit = gw_cost<CODES>(p.path[k].d) < unit ? gw_cost<CODES>(p.path[k].d) : unit;
   int grid = (p.total + 7) / 8;
   grid = grid < 148 ? grid : 148;
-  const int most = (p.total + kMaxRunGw - 1) / kMaxRunGw;
+  const int most = (int)((p.total_cost / unit + kMaxRunGw - 1) / kMaxRunGw);
   return grid < most ? most : grid;
+}
+template <bool CODES>
+int64_t gw_total_cost(const LParams& p) {
+  int64_t cost = 0;
+  for (int k = 0; k < p.num_paths; ++k)
+    for (int c = 0; c < p.num_classes; ++c) cost += (int64_t)gw_cost<CODES>(p.path[k].d) * ((p.bounds[c + 1] - p.bounds[c] + rows_per_block(p.path[k].d) - 1) / rows_per_block(p.path[k].d));
+  return cost;
+}
+// the larger of the two ways to divide the blocks, so that one size of `parts` serves both
+int gw_most_blocks(LParams& p) {
+  p.total_cost = gw_total_cost<true>(p);
+  const int a = gw_blocks<true>(p);
+  p.total_cost = gw_total_cost<false>(p);
+  const int b = gw_blocks<false>(p);
+  return a > b ? a : b;
 }
 int64_t gw_slot(const LParams& p) {
   int64_t slot = 0;
@@ -717,7 +756,7 @@ int64_t gw_floats(const LParams& p, int grid) { return (int64_t)(grid + p.num_pa
 extern "C" int64_t cueq_b200_linear_gw_floats(const cueq_linear_args* a) {
   LParams p;
   if (make_params(a, rows_per_block, true, &p)) return -1;
-  return p.total == 0 ? 0 : gw_floats(p, gw_blocks(p));
+  return p.total == 0 ? 0 : gw_floats(p, gw_most_blocks(p));
 }
 
 extern "C" int cueq_b200_linear_map(const cueq_linear_args* a, void* stream) {
@@ -738,39 +777,62 @@ extern "C" int cueq_b200_linear_map(const cueq_linear_args* a, void* stream) {
 
 namespace {
 
-// x rows -> codes and steps, a warp per row and irrep: per block of u * d values the smallest power of two of which 127 hold the
-// largest magnitude (as in norm_kernels.cuh; NaN for a block that holds an infinity or NaN).  268 MB in, 67 MB out for 32,768 nodes
-// of 128x(0e+1o+2e+3o).
+// x rows -> codes and steps: per block of u * d values the smallest power of two of which 127 hold the largest magnitude (code_step in
+// common.cuh).  A lane holds up to seven 16-byte pieces: one row of 896 values per warp, seven of 128.  268 MB in, 67 MB out for 32,768 nodes of
+// 128x(0e+1o+2e+3o).
 struct PackParams {
   const float* x;
   signed char* codes;
   float* steps;
   int64_t ldx, ldc, ld_steps, rows;
   int num_paths;
-  struct { int off, n, code_off; } path[kMaxPaths];
+  struct { int off, n, code_off; int64_t block0; } path[kMaxPaths];   // block0: first thread block
 };
 constexpr int kPackWarps = 8;
-__global__ void __launch_bounds__(32 * kPackWarps) linear_pack_kernel(const __grid_constant__ PackParams p) {
-  const int k = blockIdx.x % p.num_paths, lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)(blockIdx.x / p.num_paths) * kPackWarps + (threadIdx.x >> 5);
-  if (row >= p.rows) return;
-  const int n4 = p.path[k].n / 4;                                    // 224 at most
-  const float4* src = reinterpret_cast<const float4*>(p.x + row * p.ldx + p.path[k].off);
-  float4 v[7];
-  unsigned top = 0;
+constexpr int pack_rows(int n) { return 7 / ((n + 127) / 128); }      // rows of n values per warp
+template <int J>                                                      // pieces of a row per lane
+__device__ __forceinline__ void pack_rows_of(const PackParams& p, int k, int64_t row0, int lane) {
+  constexpr int R = 7 / J;
+  const int n4 = p.path[k].n / 4;
+  float4 v[R][J];
 #pragma unroll
-  for (int j = 0; j < 7; ++j) v[j] = lane + 32 * j < n4 ? __ldg(src + lane + 32 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const float4* src = reinterpret_cast<const float4*>(p.x + (row0 + r) * p.ldx + p.path[k].off);
+      v[r][j] = row0 + r < p.rows && lane + 32 * j < n4 ? __ldg(src + lane + 32 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
   auto bits = [](float f) { return __float_as_uint(f) & 0x7fffffffu; };
 #pragma unroll
-  for (int j = 0; j < 7; ++j) top = max(top, max(max(bits(v[j].x), bits(v[j].y)), max(bits(v[j].z), bits(v[j].w))));
-  float step, inv;
-  cueq::code_step(__reduce_max_sync(0xffffffffu, top), step, inv);
-  char4* dst = reinterpret_cast<char4*>(p.codes + row * p.ldc + p.path[k].code_off);
+  for (int r = 0; r < R; ++r) {
+    if (row0 + r >= p.rows) break;
+    unsigned top = 0;
 #pragma unroll
-  for (int j = 0; j < 7; ++j)
-    if (lane + 32 * j < n4)
-      dst[lane + 32 * j] = make_char4(cueq::to_code(v[j].x, inv), cueq::to_code(v[j].y, inv), cueq::to_code(v[j].z, inv), cueq::to_code(v[j].w, inv));
-  if (lane == 0) p.steps[k * p.ld_steps + row] = step;
+    for (int j = 0; j < J; ++j) top = max(top, max(max(bits(v[r][j].x), bits(v[r][j].y)), max(bits(v[r][j].z), bits(v[r][j].w))));
+    float step, inv;
+    cueq::code_step(__reduce_max_sync(0xffffffffu, top), step, inv);
+    char4* dst = reinterpret_cast<char4*>(p.codes + (row0 + r) * p.ldc + p.path[k].code_off);
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+      if (lane + 32 * j < n4)
+        dst[lane + 32 * j] = make_char4(cueq::to_code(v[r][j].x, inv), cueq::to_code(v[r][j].y, inv), cueq::to_code(v[r][j].z, inv), cueq::to_code(v[r][j].w, inv));
+    if (lane == 0) p.steps[k * p.ld_steps + row0 + r] = step;
+  }
+}
+__global__ void __launch_bounds__(32 * kPackWarps) linear_pack_kernel(const __grid_constant__ PackParams p) {
+  int k = 0;
+  while (k + 1 < p.num_paths && blockIdx.x >= p.path[k + 1].block0) ++k;
+  const int lane = threadIdx.x & 31;
+  const int64_t warp = (blockIdx.x - p.path[k].block0) * kPackWarps + (threadIdx.x >> 5);
+  switch ((p.path[k].n + 127) / 128) {                                // u * d <= 896
+    case 1: pack_rows_of<1>(p, k, warp * 7, lane); break;
+    case 2: pack_rows_of<2>(p, k, warp * 3, lane); break;
+    case 3: pack_rows_of<3>(p, k, warp * 2, lane); break;
+    case 4: pack_rows_of<4>(p, k, warp, lane); break;
+    case 5: pack_rows_of<5>(p, k, warp, lane); break;
+    case 6: pack_rows_of<6>(p, k, warp, lane); break;
+    default: pack_rows_of<7>(p, k, warp, lane); break;
+  }
 }
 
 // blocks of codes in the order of the paths, one behind the other; multiples of 32 bytes each
@@ -805,13 +867,17 @@ extern "C" int cueq_b200_linear_pack(const cueq_linear_args* a, const cueq_linea
   if (int rc = make_params(a, rows_per_block, true, &p)) return rc;
   if (int rc = check_codes(a, c, off)) return rc;
   if (c->rows == 0) return 0;
-  const int64_t groups = (c->rows + kPackWarps - 1) / kPackWarps;
-  if (groups * a->num_paths > 2147483647LL) return cueq::fail("linear: too many rows");
   PackParams q;
   q.x = p.x; q.codes = (signed char*)c->codes; q.steps = (float*)c->steps;
   q.ldx = p.ldx; q.ldc = c->ld_codes; q.ld_steps = c->ld_steps; q.rows = c->rows; q.num_paths = a->num_paths;
-  for (int k = 0; k < a->num_paths; ++k) { q.path[k].off = a->paths[k].x_off; q.path[k].n = a->paths[k].u * a->paths[k].d; q.path[k].code_off = off[k]; }
-  linear_pack_kernel<<<(unsigned)(groups * a->num_paths), 32 * kPackWarps, 0, reinterpret_cast<cudaStream_t>(stream)>>>(q);
+  int64_t blocks = 0;
+  for (int k = 0; k < a->num_paths; ++k) {
+    const int n = a->paths[k].u * a->paths[k].d, per_block = kPackWarps * pack_rows(n);
+    q.path[k].off = a->paths[k].x_off; q.path[k].n = n; q.path[k].code_off = off[k]; q.path[k].block0 = blocks;
+    blocks += (c->rows + per_block - 1) / per_block;
+  }
+  if (blocks > 2147483647LL) return cueq::fail("linear: too many rows");
+  linear_pack_kernel<<<(unsigned)blocks, 32 * kPackWarps, 0, reinterpret_cast<cudaStream_t>(stream)>>>(q);
   CUEQ_CUDA_OK(cudaGetLastError());
   return 0;
 }
@@ -831,7 +897,8 @@ int launch_gw(const cueq_linear_args* a, const cueq_linear_codes* codes, void* s
   p.g = (const float*)a->w;
   p.out = (float*)a->out;
   if (p.total == 0) return 0;
-  const int grid = gw_blocks(p);
+  p.total_cost = codes ? gw_total_cost<true>(p) : gw_total_cost<false>(p);
+  const int grid = codes ? gw_blocks<true>(p) : gw_blocks<false>(p);
   const int64_t need = gw_floats(p, grid);
   if (!a->parts || a->parts_floats < need || ((uintptr_t)a->parts & 15))
     return cueq::fail("linear: the weight gradient needs room for %lld floats of partial sums, 16-byte aligned", (long long)need);
@@ -839,12 +906,14 @@ int launch_gw(const cueq_linear_args* a, const cueq_linear_codes* codes, void* s
   p.slot = gw_slot(p);
   GwStarts t;
   int widest = 0;
-  for (int k = 0, s = 0, at = 0; k < p.num_paths; ++k) {
+  int64_t at = 0;
+  for (int k = 0, s = 0; k < p.num_paths; ++k) {
     widest = p.path[k].K * p.path[k].N > widest ? p.path[k].K * p.path[k].N : widest;
     const int n = rows_per_block(p.path[k].d);
+    t.cost[k] = codes ? gw_cost<true>(p.path[k].d) : gw_cost<false>(p.path[k].d);
     for (int c = 0; c < p.num_classes; ++c, ++s) {
       t.start[s] = at;
-      at += (p.bounds[c + 1] - p.bounds[c] + n - 1) / n;
+      at += (int64_t)t.cost[k] * ((p.bounds[c + 1] - p.bounds[c] + n - 1) / n);
       t.start[s + 1] = at;
     }
   }
