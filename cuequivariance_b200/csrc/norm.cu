@@ -26,7 +26,7 @@ int check(const cueq_norm_args* a) {
   if (a->num_blocks < 1 || a->num_blocks > kMaxBlocks || !a->blocks) return cueq::fail("norm: between 1 and %d irrep blocks", kMaxBlocks);
   if (a->rows < 0 || a->rows >= (int64_t(1) << 40)) return cueq::fail("norm: bad number of rows");
   for (int k = 0; k < a->num_blocks; ++k)
-    if (a->blocks[k].mul < 1 || a->blocks[k].dim < 1 || (int64_t)a->blocks[k].mul * a->blocks[k].dim > (1 << 24)) return cueq::fail("norm: bad irrep block %d", k);
+    if (a->blocks[k].mul < 1 || a->blocks[k].dim < 1 || a->blocks[k].dim > 32767 || (int64_t)a->blocks[k].mul * a->blocks[k].dim > (1 << 24)) return cueq::fail("norm: bad irrep block %d", k);
   if (a->stats_stride && a->stats_stride != 8 && (a->stats_stride != 4 || (a->codes && a->mode == kBoth))) return cueq::fail("norm: bad stride of the statistics");
   if (!(a->eps > 0)) return cueq::fail("norm: eps must be positive");
   if (a->codes && a->dtype == CUEQ_F64) return cueq::fail("norm: 64-bit data are not kept in 8 bits");
@@ -101,7 +101,7 @@ int make_plan(const cueq_norm_args* a, bool backward, bool dense, Params* p, int
   bool even = true;
   for (int k = 0; k < a->num_blocks; ++k) {
     Blk& b = p->blk[k];
-    b.mul = a->blocks[k].mul; b.dim = a->blocks[k].dim;
+    b.mul = a->blocks[k].mul; b.dim = (short)a->blocks[k].dim;
     b.off = p->dim_total; b.ch = p->channels;
     const int n = b.mul * b.dim;
     if (!ns || p->slice[ns - 1].values + n > kSliceValues) { p->slice[ns] = Slice{}; p->slice[ns].first = k; ++ns; }
@@ -116,7 +116,24 @@ int make_plan(const cueq_norm_args* a, bool backward, bool dense, Params* p, int
   int unit = 1;                                          // rows after which dense rows are on a 16-byte boundary again
   if (dense && ns == 1) while (unit < 8 && (unit * p->dim_total * size % 16 || (gated(a) && unit * p->channels * size % 16))) unit *= 2;
   auto stage = [&](const Slice& s) { return backward ? backward_stage(*p, s, a->mode, q8, size, stat).total : forward_stage(*p, s, a->mode, q8, size).total; };
-  auto need = [&](const Slice& s, int stages) { return head_bytes(msize, s.channels, backward) + stages * stage(s); };
+  auto need = [&](const Slice& s, int stages) { return head_bytes(msize, s, backward) + stages * stage(s); };
+  // How a block is worked on: up to 32, 64 or 128 channels by 1, 2 or 4 per lane, where these are neighbours on a boundary of as many
+  // values in every row; up to 16 channels with several rows side by side.  The rest, l > 3 among it, goes through loops (256 channels: 0.6
+  // of the copy bandwidth where 128 have 0.75).
+  for (int q = 0; q < ns; ++q) {
+    Slice& s = p->slice[q];
+    const Blk& b0 = p->blk[s.first];
+    for (int k = s.first; k < s.first + s.count; ++k) {
+      Blk& b = p->blk[k];
+      const int per = b.mul <= 32 ? 1 : b.mul <= 64 ? 2 : 4;
+      const int places = (b.off - b0.off) | (b.ch - b0.ch) | b.mul | s.values | s.channels;
+      b.per_lane = b.dim <= 7 && b.dim % 2 && b.mul <= 128 && places % per == 0 ? per : 0;
+      b.lanes = 32;
+      while (b.per_lane == 1 && b.lanes / 2 >= b.mul) b.lanes /= 2;
+      b.sum = s.sums;
+      s.sums += pad4(b.lanes < 32 ? 32 : b.mul);
+    }
+  }
   p->stages = 2;
   p->unit = unit;
   int smem = 0;
@@ -127,7 +144,7 @@ int make_plan(const cueq_norm_args* a, bool backward, bool dense, Params* p, int
     if (need(s, 2) > kSmemPerSm) p->stages = 1;
     const int one = stage(s) / unit;
     int rps = kStageBytes / (one ? one : 1) / unit * unit;
-    rps = rps >= 3 ? (rps + 1) & ~3 : rps;               // rows are worked on by fours, twos or one by one
+    rps = rps >= 3 ? (rps + 1) / 4 * 4 : rps;            // rows are worked on by fours, twos or one by one
     s.rps = rps < unit ? unit : rps > 32 ? 32 : rps;
     while (s.rps > unit && copy_lanes(a, backward, *p, s.rps) > 32) s.rps -= unit;
   }

@@ -40,12 +40,16 @@ __host__ __device__ constexpr int warps_per_sm(int msize) { return msize == 8 ? 
 enum Mode { kBranch = 1, kNorm = 2, kBoth = 3 };
 
 struct Blk {
-  int mul, dim, off, ch;             // off, ch: first element of the block in a row of features, first channel
+  int mul, off, ch;                  // off, ch: first element of the block in a row of features, first channel
   int code, gcode, hcode;            // first byte in a row of codes: of y (or x, norm alone), of the gates, of h
+  int sum;                           // first of its sums, in those of the slice
+  short dim;
+  unsigned char per_lane, lanes;     // neighbouring channels of a lane (0: any number, one by one), lanes of a row
 };
 struct Slice {
   int first, count;                  // blocks
   int values, channels;              // their elements and channels
+  int sums;                          // sums per parameter: one per channel, or per channel of every row that a warp takes at a time
   int rps;                           // rows per stage
 };
 // How rows of an operand move.  kRows: a bulk copy per row; kDense: rows follow one another without a gap, one bulk copy per stage;
@@ -134,7 +138,8 @@ __host__ __device__ inline Stage backward_stage(const Params& p, const Slice& s,
 }
 // in front of the stages: 2 barriers and the tensors' moves; per channel s, w, s act(g) of the row at work, and (backward) the sums of both gradients
 constexpr int kMoves = 11, kMoveBytes = 40, kBars = 16 + kMoves * kMoveBytes + 8;
-__host__ __device__ inline int head_bytes(int msize, int channels, bool backward) { return (kBars + msize * channels * (backward ? 5 : 3) + 127) & ~127; }
+__host__ __device__ constexpr int pad4(int n) { return (n + 3) & ~3; }
+__host__ __device__ inline int head_bytes(int msize, const Slice& s, bool backward) { return (kBars + msize * (3 * pad4(s.channels) + (backward ? 2 * s.sums : 0)) + 127) & ~127; }
 
 // ---- conversions ----------------------------------------------------------------------------------------------------
 template <class M> __device__ __forceinline__ M to(float v) { return (M)v; }
@@ -174,7 +179,7 @@ __device__ __forceinline__ signed char to_code(double, float) { return 0; }
 template <class M>
 struct View {
   M *s, *w, *a, *acc_s, *acc_w;      // parameters, s act(g), sums; per channel of the block
-  int mul, dim, lane, gate, gated;
+  int mul, dim, lane, lanes, gate, gated;
   M inv_n, eps;
 };
 
@@ -330,9 +335,12 @@ __device__ __forceinline__ void backward_item(const View<M>& c, T* __restrict__ 
   }
 }
 
-// ---- R rows of one irrep block of 32 K channels, K <= 4, in registers -----------------------------------------------------------------
-// Read from shared memory once, written once.  Short blocks take several rows at a time: what a call costs besides its values, above all the
-// sums over the warp, is most of their time.  Of fewer than R rows the last one is read in place of the missing ones.
+// ---- rows of an irrep block whose values a warp holds in registers ------------------------------------------------------------------------
+// A lane owns K = 1, 2 or 4 neighbouring channels: K * DIM values, moved as DIM vectors of K values in either layout (mul_ir: one behind the
+// other; no bank conflicts, DIM is odd).  Shared memory is read once and written once, an instruction for K values.
+//
+// Short blocks take several rows at a time, as what a call costs besides its values, above all the sums over the warp, is most of their
+// time: R rows per lane, or (NARROW, up to 16 channels) a row per `lanes` lanes.  Of missing rows and channels the last one is read instead.
 template <int DIM, int K> constexpr int kRowsAtOnce = DIM * K <= 2 ? 4 : DIM * K <= 8 ? 2 : 1;
 
 // rows of one region: E at byte `base`, `pitch` bytes apart
@@ -342,14 +350,18 @@ struct Rows {
   int pitch;
   __device__ __forceinline__ E* operator[](int q) const { return reinterpret_cast<E*>(base + q * pitch); }
 };
+template <class E, int K>
+struct alignas(sizeof(E) * K < 16 ? sizeof(E) * K : 16) Vec { E v[K]; };
 
-// sums of R values each over the warp, every one by the same pairs in the same order as cueq::warp_sum
-template <int R, class M>
-__device__ __forceinline__ void warp_sums(M (&s)[R], int lane) {
-  if constexpr (R == 1) {
+// sums of R values each over the warp, every one by the same pairs in the same order as cueq::warp_sum; NARROW: over `lanes` lanes
+template <bool NARROW, int R, class M>
+__device__ __forceinline__ void warp_sums(M (&s)[R], int lane, int lanes) {
+  constexpr unsigned all = 0xffffffffu;
+  if constexpr (NARROW) {
+    for (int o = lanes >> 1; o; o >>= 1) s[0] += __shfl_xor_sync(all, s[0], o);
+  } else if constexpr (R == 1) {
     s[0] = cueq::warp_sum(s[0]);
   } else {
-    constexpr unsigned all = 0xffffffffu;
     M t;
     if constexpr (R == 2) {
       const bool up = lane & 16;
@@ -366,36 +378,84 @@ __device__ __forceinline__ void warp_sums(M (&s)[R], int lane) {
     for (int q = 0; q < R; ++q) s[q] = __shfl_sync(all, t, (q & 1) * 16 + (q >> 1) * 8);
   }
 }
+template <bool NARROW>
+__device__ __forceinline__ unsigned warp_top(unsigned v, int lanes) {
+  if (!NARROW) return __reduce_max_sync(0xffffffffu, v);
+  for (int o = lanes >> 1; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
 
-template <class T, class M, int DIM, bool MUL_IR, int K, int R>
+template <class T, class M, int DIM, bool MUL_IR, int K, int R, bool NARROW>
 struct Short {
-  int lane, mul, left;               // left: rows that there are, 1 .. R
-  __device__ __forceinline__ int row(int q) const { return R == 1 ? 0 : min(q, left - 1); }
-  __device__ __forceinline__ bool there(int q) const { return R == 1 || q < left; }
-  __device__ __forceinline__ int at(int k, int i) const { return MUL_IR ? (lane + 32 * k) * DIM + i : i * mul + lane + 32 * k; }
+  int lane, lanes, first, mul, left; // first: this lane's vector of channels; left: rows that there are, from 1 on
+  int group;                         // NARROW: this lane's row
+  bool on;                           // the lane has channels
+  __device__ __forceinline__ Short(const View<M>& c, int left_) : lane(c.lane), lanes(c.lanes), mul(c.mul), left(left_) {
+    const int l = NARROW ? lane % lanes : lane;
+    group = NARROW ? lane / lanes : 0;
+    on = l * K < mul;
+    first = on ? l : 0;
+  }
+  __device__ __forceinline__ int row(int q) const { return NARROW ? min(group, left - 1) : R == 1 ? 0 : min(q, left - 1); }
+  __device__ __forceinline__ bool there(int q) const { return on && (NARROW ? group < left : R == 1 || q < left); }
+  // vector j of DIM, in vectors
+  __device__ __forceinline__ int at(int j) const { return MUL_IR ? first * DIM + j : j * (mul / K) + first; }
   template <class E>
   __device__ __forceinline__ void load(const Rows<E>& p, M (&v)[R][K][DIM]) const {
 #pragma unroll
     for (int q = 0; q < R; ++q) {
-      const E* e = p[row(q)];
+      const Vec<E, K>* e = reinterpret_cast<const Vec<E, K>*>(p[row(q)]);
 #pragma unroll
-      for (int k = 0; k < K; ++k)
+      for (int j = 0; j < DIM; ++j) {
+        const Vec<E, K> x = e[at(j)];
 #pragma unroll
-        for (int i = 0; i < DIM; ++i) v[q][k][i] = to<M>(e[at(k, i)]);
+        for (int k = 0; k < K; ++k) {
+          if (MUL_IR) v[q][(j * K + k) / DIM][(j * K + k) % DIM] = to<M>(x.v[k]);
+          else v[q][k][j] = to<M>(x.v[k]);
+        }
+      }
+    }
+  }
+  template <class E, class F>
+  __device__ __forceinline__ void put(E* row, const M (&v)[K][DIM], F convert) const {
+    Vec<E, K>* e = reinterpret_cast<Vec<E, K>*>(row);
+#pragma unroll
+    for (int j = 0; j < DIM; ++j) {
+      Vec<E, K> x;
+#pragma unroll
+      for (int k = 0; k < K; ++k) x.v[k] = convert(MUL_IR ? v[(j * K + k) / DIM][(j * K + k) % DIM] : v[k][j]);
+      e[at(j)] = x;
     }
   }
   __device__ __forceinline__ void store(const Rows<T>& p, const M (&v)[R][K][DIM]) const {
 #pragma unroll
-    for (int q = 0; q < R; ++q) {
-      if (!there(q)) break;
-      T* e = p[q];
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < DIM; ++i) e[at(k, i)] = from<T>(v[q][k][i]);
-    }
+    for (int q = 0; q < R; ++q)
+      if (there(q)) put(p[row(q)], v[q], [](M m) { return from<T>(m); });
   }
-  // steps of R rows, and their codes
+  // K values of a row of channels
+  template <class E>
+  __device__ __forceinline__ void channels(const E* row, M (&v)[K]) const {
+    const Vec<E, K> x = reinterpret_cast<const Vec<E, K>*>(row)[first];
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = to<M>(x.v[k]);
+  }
+  template <class E, class F>
+  __device__ __forceinline__ void put_channels(E* row, const M (&v)[K], F convert) const {
+    Vec<E, K> x;
+#pragma unroll
+    for (int k = 0; k < K; ++k) x.v[k] = convert(v[k]);
+    reinterpret_cast<Vec<E, K>*>(row)[first] = x;
+  }
+  // this lane's sums of its channels, one set per lane (NARROW) or channel
+  __device__ __forceinline__ void add(M* sums, const M (&v)[K]) const {
+    if (!on) return;
+    Vec<M, K>* e = reinterpret_cast<Vec<M, K>*>(sums) + (NARROW ? lane : first);
+    Vec<M, K> x = *e;
+#pragma unroll
+    for (int k = 0; k < K; ++k) x.v[k] += v[k];
+    *e = x;
+  }
+  // steps of the rows, and their codes
   __device__ __forceinline__ void code(const Rows<signed char>& p, const M (&v)[R][K][DIM], float (&step)[R]) const {
 #pragma unroll
     for (int q = 0; q < R; ++q) {
@@ -405,16 +465,11 @@ struct Short {
 #pragma unroll
         for (int i = 0; i < DIM; ++i) t = max(t, magnitude(v[q][k][i]));
       float inverse;
-      code_step(__reduce_max_sync(0xffffffffu, t), step[q], inverse);
-      if (!there(q)) continue;
-      signed char* e = p[q];
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < DIM; ++i) e[at(k, i)] = to_code(v[q][k][i], inverse);
+      code_step(warp_top<NARROW>(t, lanes), step[q], inverse);
+      if (there(q)) put(p[row(q)], v[q], [=](M m) { return to_code(m, inverse); });
     }
   }
-  // r of R rows
+  // r of the rows
   __device__ __forceinline__ void inverse_rms(const M (&v)[R][K][DIM], M inv_n, M eps, M (&r)[R]) const {
 #pragma unroll
     for (int q = 0; q < R; ++q) {
@@ -427,56 +482,48 @@ struct Short {
         for (int i = 0; i < DIM; ++i) part[i] += v[q][k][i] * v[q][k][i];
 #pragma unroll
       for (int i = 1; i < DIM; ++i) part[0] += part[i];
-      r[q] = part[0];
+      r[q] = on ? part[0] : M(0);
     }
-    warp_sums(r, lane);
+    warp_sums<NARROW>(r, lane, lanes);
 #pragma unroll
     for (int q = 0; q < R; ++q) r[q] = inverse_sqrt(r[q] * inv_n + eps);
   }
+  __device__ __forceinline__ bool leads() const { return NARROW ? lane % lanes == 0 : lane == 0; }
 };
 
-template <class T, class M, int MODE, bool Q8, int DIM, bool MUL_IR, int K, int R>
+template <class T, class M, int MODE, bool Q8, int DIM, bool MUL_IR, int K, int R, bool NARROW>
 __device__ __forceinline__ void forward_short(const View<M>& c, int left, Rows<T> x, Rows<T> y, Rows<T> g, Rows<signed char> ca, Rows<signed char> cg,
                                               Rows<signed char> ch, M* stats, int64_t ld_stats) {
-  const Short<T, M, DIM, MUL_IR, K, R> w{c.lane, c.mul, left};
-  M v[R][K][DIM], xv[R][K][DIM], a[R][K], r[R], rh[R];
+  const Short<T, M, DIM, MUL_IR, K, R, NARROW> w(c, left);
+  M v[R][K][DIM], xv[R][K][DIM], a[R][K], r[R], rh[R], s[K];
   float step[R], gstep[R], hstep[R];
   w.load((MODE & kBranch) ? y : x, v);
   if (MODE & kBranch) w.load(x, xv);
+  w.channels((MODE & kBranch) ? c.s : c.w, s);
 #pragma unroll
   for (int q = 0; q < R; ++q) {
     gstep[q] = 0.f;
     if ((MODE & kBranch) && c.gated) {
-      const T* e = g[w.row(q)];
       M gate[K];
-#pragma unroll
-      for (int k = 0; k < K; ++k) gate[k] = to<M>(e[c.lane + 32 * k]);
+      w.channels(g[w.row(q)], gate);
       if (Q8) {
         unsigned top = 0;
         float inverse;
 #pragma unroll
         for (int k = 0; k < K; ++k) top = max(top, magnitude(gate[k]));
-        code_step(__reduce_max_sync(0xffffffffu, top), gstep[q], inverse);
-        if (w.there(q)) {
-#pragma unroll
-          for (int k = 0; k < K; ++k) cg[q][c.lane + 32 * k] = to_code(gate[k], inverse);
-        }
+        code_step(warp_top<NARROW>(top, w.lanes), gstep[q], inverse);
+        if (w.there(q)) w.put_channels(cg[w.row(q)], gate, [=](M m) { return to_code(m, inverse); });
       }
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        M de;
-        activation(c.gate, gate[k], a[q][k], de);
+        M e, de;
+        activation(c.gate, gate[k], e, de);
+        a[q][k] = s[k] * e;
       }
     } else {
 #pragma unroll
-      for (int k = 0; k < K; ++k) a[q][k] = M(1);
+      for (int k = 0; k < K; ++k) a[q][k] = s[k];
     }
-  }
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const M s = ((MODE & kBranch) ? c.s : c.w)[c.lane + 32 * k];
-#pragma unroll
-    for (int q = 0; q < R; ++q) a[q][k] *= s;
   }
   w.inverse_rms(v, c.inv_n, c.eps, r);
   if (Q8) w.code(ca, v, step);
@@ -490,21 +537,20 @@ __device__ __forceinline__ void forward_short(const View<M>& c, int left, Rows<T
   if (MODE == kBoth) {
     w.inverse_rms(v, c.inv_n, c.eps, rh);
     if (Q8) w.code(ch, v, hstep);
+    w.channels(c.w, s);
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const M b = c.w[c.lane + 32 * k];
+    for (int q = 0; q < R; ++q)
 #pragma unroll
-      for (int q = 0; q < R; ++q)
+      for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < DIM; ++i) v[q][k][i] *= b * rh[q];
-    }
+        for (int i = 0; i < DIM; ++i) v[q][k][i] *= s[k] * rh[q];
     w.store(y, v);
   }
-  if (stats && c.lane == 0) {
+  if (stats && w.leads()) {
 #pragma unroll
     for (int q = 0; q < R; ++q) {
       if (!w.there(q)) break;
-      M* e = stats + q * ld_stats;
+      M* e = stats + w.row(q) * ld_stats;
       e[0] = r[q];
       if (MODE == kBoth) e[1] = rh[q];
       if (Q8) { e[2] = M(step[q]); e[3] = M(gstep[q]); }
@@ -513,17 +559,18 @@ __device__ __forceinline__ void forward_short(const View<M>& c, int left, Rows<T
   }
 }
 
-template <class T, class M, class K8, int MODE, bool Q8, int DIM, bool MUL_IR, int K, int R>
+template <class T, class M, class K8, int MODE, bool Q8, int DIM, bool MUL_IR, int K, int R, bool NARROW>
 __device__ __forceinline__ void backward_short(const View<M>& c, int left, Rows<T> go, Rows<T> gn, Rows<K8> h, Rows<K8> y, Rows<K8> g, Rows<T> dg,
                                                Rows<M> stats, bool has_go) {
-  const Short<T, M, DIM, MUL_IR, K, R> w{c.lane, c.mul, left};
-  M o[R][K][DIM], v[R][K][DIM], dot[R];
+  const Short<T, M, DIM, MUL_IR, K, R, NARROW> w(c, left);
+  M o[R][K][DIM], v[R][K][DIM], dot[R], sum[K];
   if (MODE & kNorm) {
-    M rh[R], step[R], p[R][K], b[K];
+    M rh[R], step[R], b[K];
     w.load(gn, o);
     w.load(h, v);
+    w.channels(c.w, b);
 #pragma unroll
-    for (int k = 0; k < K; ++k) b[k] = c.w[c.lane + 32 * k];
+    for (int k = 0; k < K; ++k) sum[k] = M(0);
 #pragma unroll
     for (int q = 0; q < R; ++q) {
       const M* e = stats[w.row(q)];
@@ -532,21 +579,17 @@ __device__ __forceinline__ void backward_short(const View<M>& c, int left, Rows<
       dot[q] = M(0);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        p[q][k] = M(0);
+        M p = M(0);
 #pragma unroll
-        for (int i = 0; i < DIM; ++i) p[q][k] += o[q][k][i] * v[q][k][i];
-        p[q][k] *= rh[q] * step[q];
-        dot[q] += b[k] * p[q][k];
+        for (int i = 0; i < DIM; ++i) p += o[q][k][i] * v[q][k][i];
+        p *= rh[q] * step[q];
+        sum[k] += w.there(q) ? p : M(0);
+        dot[q] += b[k] * p;
       }
+      dot[q] = w.on ? dot[q] : M(0);
     }
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      M sum = c.acc_w[c.lane + 32 * k];
-#pragma unroll
-      for (int q = 0; q < R; ++q) sum += w.there(q) ? p[q][k] : M(0);
-      c.acc_w[c.lane + 32 * k] = sum;
-    }
-    warp_sums(dot, c.lane);
+    w.add(c.acc_w, sum);
+    warp_sums<NARROW>(dot, c.lane, w.lanes);
 #pragma unroll
     for (int q = 0; q < R; ++q) {
       const M qh = rh[q] * (rh[q] * (c.inv_n * dot[q])) * step[q];
@@ -572,35 +615,37 @@ __device__ __forceinline__ void backward_short(const View<M>& c, int left, Rows<
   } else {
     w.load(go, o);
   }
-  M r[R], step[R], a[R][K];
+  M r[R], step[R], a[R][K], s[K];
   w.load(y, v);
+  w.channels(c.s, s);
+#pragma unroll
+  for (int k = 0; k < K; ++k) sum[k] = M(0);
 #pragma unroll
   for (int q = 0; q < R; ++q) {
-    const M* e = stats[w.row(q)];
-    r[q] = e[0];
-    step[q] = Q8 ? e[2] : M(1);
+    const M* st = stats[w.row(q)];
+    r[q] = st[0];
+    step[q] = Q8 ? st[2] : M(1);
     dot[q] = M(0);
-  }
+    M gate[K], de[K];
+    if (c.gated) w.channels(g[w.row(q)], gate);
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int u = c.lane + 32 * k;
-    const M s = c.s[u];
-    M sum = c.acc_s[u];
-#pragma unroll
-    for (int q = 0; q < R; ++q) {
-      M e = M(1), de = M(0), p = M(0);
-      if (c.gated) activation(c.gate, to<M>(g[w.row(q)][u]) * (Q8 ? stats[w.row(q)][3] : M(1)), e, de);
+    for (int k = 0; k < K; ++k) {
+      M e = M(1), p = M(0);
+      de[k] = M(0);
+      if (c.gated) activation(c.gate, Q8 ? gate[k] * st[3] : gate[k], e, de[k]);
 #pragma unroll
       for (int i = 0; i < DIM; ++i) p += o[q][k][i] * v[q][k][i];
       p *= r[q] * step[q];
-      a[q][k] = s * e;
+      a[q][k] = s[k] * e;
       dot[q] += a[q][k] * p;
-      sum += w.there(q) ? e * p : M(0);
-      if (c.gated && w.there(q)) dg[q][u] = from<T>(s * de * p);   // may lie over g[q][u], which no later row reads
+      sum[k] += w.there(q) ? e * p : M(0);
+      de[k] *= s[k] * p;
     }
-    c.acc_s[u] = sum;
+    dot[q] = w.on ? dot[q] : M(0);
+    if (c.gated && w.there(q)) w.put_channels(dg[w.row(q)], de, [](M m) { return from<T>(m); });   // may lie over g, of which no other lane reads this
   }
-  warp_sums(dot, c.lane);
+  w.add(c.acc_s, sum);
+  warp_sums<NARROW>(dot, c.lane, w.lanes);
 #pragma unroll
   for (int q = 0; q < R; ++q) {
     const M qy = r[q] * (r[q] * (c.inv_n * dot[q])) * step[q];
@@ -758,21 +803,22 @@ __device__ __forceinline__ void init_barriers(unsigned char* smem) {
 // parameters of the slice's channels into shared memory, sums cleared
 template <class M>
 __device__ __forceinline__ void prepare(const Params& p, const Slice& s, M* at, bool backward) {
-  const int ch = p.blk[s.first].ch, n = s.channels;
-  for (int u = threadIdx.x; u < n; u += 32) {
+  const int ch = p.blk[s.first].ch, n = pad4(s.channels);
+  for (int u = threadIdx.x; u < s.channels; u += 32) {
     at[u] = p.s ? cueq::load_as<M>(p.s, p.pdtype, ch + u) : M(1);
     at[n + u] = p.w ? cueq::load_as<M>(p.w, p.pdtype, ch + u) : M(1);
-    if (backward) at[3 * n + u] = at[4 * n + u] = M(0);
   }
+  if (backward)
+    for (int u = threadIdx.x; u < 2 * s.sums; u += 32) at[3 * n + u] = M(0);
   __syncwarp();
 }
 template <class M>
 __device__ __forceinline__ View<M> block_view(const Params& p, const Slice& s, const Blk& b, M* at) {
   View<M> c;
-  const int u0 = b.ch - p.blk[s.first].ch, n = s.channels;
-  c.s = at + u0; c.w = at + n + u0; c.a = at + 2 * n + u0; c.acc_s = at + 3 * n + u0; c.acc_w = at + 4 * n + u0;
+  const int u0 = b.ch - p.blk[s.first].ch, n = pad4(s.channels);
+  c.s = at + u0; c.w = at + n + u0; c.a = at + 2 * n + u0; c.acc_s = at + 3 * n + b.sum; c.acc_w = c.acc_s + s.sums;
   c.mul = b.mul; c.dim = b.dim;
-  c.lane = threadIdx.x;
+  c.lane = threadIdx.x; c.lanes = b.lanes;
   c.gate = p.gate; c.gated = p.gate != CUEQ_NORM_GATE_NONE;
   c.inv_n = reciprocal(M(b.mul * b.dim));
   c.eps = M(p.eps);
@@ -792,12 +838,11 @@ __device__ __forceinline__ void put_moves(Move* moves, const Move (&in)[NIN], in
 
 // (dimension, channels per lane) of a block: SHORT for those that registers hold, LONG, row by row, for the others
 #define CUEQ_NORM_K(D, SHORT)                                                          \
-  if (b.mul == 32) { SHORT(D, 1); }                                                    \
-  else if (b.mul == 64) { SHORT(D, 2); }                                               \
-  else if (b.mul == 96) { SHORT(D, 3); }                                               \
-  else { SHORT(D, 4); }
+  if (b.per_lane == 4) { SHORT(D, 4) }                                                 \
+  else if (b.per_lane == 2) { SHORT(D, 2) }                                            \
+  else { SHORT(D, 1) }
 #define CUEQ_NORM_DIMS(SHORT, LONG)                                                    \
-  if (b.mul <= 128 && b.mul % 32 == 0 && b.dim <= 7) {                                 \
+  if (b.per_lane) {                                                                    \
     switch (b.dim) {                                                                   \
       case 1: CUEQ_NORM_K(1, SHORT) break;                                             \
       case 3: CUEQ_NORM_K(3, SHORT) break;                                             \
@@ -813,6 +858,11 @@ __device__ __forceinline__ void put_moves(Move* moves, const Move (&in)[NIN], in
       default: LONG(0) break;                                                          \
     }                                                                                  \
   }
+// one row at a time, several per lane, or several side by side
+#define CUEQ_SHORT(D, N)                                                                                               \
+  if (N == 1 && b.lanes < 32) { CUEQ_ROWS(D, 1, 1, true, 32 / b.lanes) }                                               \
+  else if (kRowsAtOnce<D, N> > 1 && n > 1) { CUEQ_ROWS(D, N, (kRowsAtOnce<D, N>), false, (kRowsAtOnce<D, N>)) }        \
+  else { CUEQ_ROWS(D, N, 1, false, 1) }
 
 template <class T, class M, int MODE, bool Q8, bool MUL_IR>
 __device__ __forceinline__ bool forward_slice(const Params& p, const Slice& sl, int64_t first, int64_t last, unsigned char* smem, unsigned& phases) {
@@ -837,7 +887,7 @@ __device__ __forceinline__ bool forward_slice(const Params& p, const Slice& sl, 
   const int nout = 1 + (MODE == kBoth) + (Q8 ? 1 + (MODE == kBoth) + gated : 0);
   const int nin = (MODE & kBranch) ? 2 + gated : 1;
   put_moves(moves, in, nin, out, nout);
-  return run_stages(p, sl.rps, first, last, moves, nin, moves + nin, nout, smem + head_bytes(sizeof(M), sl.channels, false), st.total,
+  return run_stages(p, sl.rps, first, last, moves, nin, moves + nin, nout, smem + head_bytes(sizeof(M), sl, false), st.total,
                     reinterpret_cast<unsigned long long*>(smem), phases, [&]() { prepare<M>(p, sl, at, false); }, [&](unsigned char* s, int64_t z, int n) {
     for (int k = sl.first; k < sl.first + sl.count; ++k) {
       const Blk& b = p.blk[k];
@@ -850,20 +900,15 @@ __device__ __forceinline__ bool forward_slice(const Params& p, const Slice& sl, 
       const int64_t ld_stats = (int64_t)p.nb * p.ns;
       M* stats = p.stats ? reinterpret_cast<M*>(p.stats) + z * ld_stats + k * p.ns : nullptr;
       auto rows_on = [](auto t, int r) { t.base += r * t.pitch; return t; };
-#define CUEQ_ROWS(D, N, R)                                                                                                             \
-  for (int r = 0; r < n; r += R)                                                                                                       \
-    forward_short<T, M, MODE, Q8, D, MUL_IR, N, R>(c, n - r, rows_on(rx, r), rows_on(ry, r), rows_on(rg, r), rows_on(ra, r), rows_on(rc, r), \
-                                                   rows_on(rh, r), stats ? stats + r * ld_stats : nullptr, ld_stats);
-#define CUEQ_SHORT(D, N)                                                                                                               \
-  if constexpr (kRowsAtOnce<D, N> > 1) {                                                                                               \
-    if (n > 1) { CUEQ_ROWS(D, N, (kRowsAtOnce<D, N>)) } else { CUEQ_ROWS(D, N, 1) }                                                    \
-  } else { CUEQ_ROWS(D, N, 1) }
+#define CUEQ_ROWS(D, N, R, NARROW, STEP)                                                                                                \
+  for (int r = 0; r < n; r += STEP)                                                                                                    \
+    forward_short<T, M, MODE, Q8, D, MUL_IR, N, R, NARROW>(c, n - r, rows_on(rx, r), rows_on(ry, r), rows_on(rg, r), rows_on(ra, r),     \
+                                                           rows_on(rc, r), rows_on(rh, r), stats ? stats + r * ld_stats : nullptr, ld_stats);
 #define CUEQ_LONG(D)                                                                                                                   \
   for (int r = 0; r < n; ++r)                                                                                                          \
     forward_item<T, M, MODE, Q8, D, MUL_IR>(c, rx[r], ry[r], rg[r], ra[r], rc[r], rh[r], stats ? stats + r * ld_stats : nullptr);
       CUEQ_NORM_DIMS(CUEQ_SHORT, CUEQ_LONG)
 #undef CUEQ_LONG
-#undef CUEQ_SHORT
 #undef CUEQ_ROWS
     }
   });
@@ -901,7 +946,7 @@ __device__ __forceinline__ bool backward_slice(const Params& p, const Slice& sl,
   const Move out[3] = {MODE == kNorm ? o_b : o_a, MODE == kBoth ? o_b : o_g, o_g};
   const int nout = MODE == kNorm ? 1 : 1 + (MODE == kBoth) + gated;
   put_moves(moves, in, nin, out, nout);
-  const bool done = run_stages(p, sl.rps, first, last, moves, nin, moves + nin, nout, smem + head_bytes(sizeof(M), sl.channels, true), st.total,
+  const bool done = run_stages(p, sl.rps, first, last, moves, nin, moves + nin, nout, smem + head_bytes(sizeof(M), sl, true), st.total,
                                reinterpret_cast<unsigned long long*>(smem), phases, [&]() { prepare<M>(p, sl, at, true); }, [&](unsigned char* s, int64_t, int n) {
     for (int k = sl.first; k < sl.first + sl.count; ++k) {
       const Blk& b = p.blk[k];
@@ -914,27 +959,29 @@ __device__ __forceinline__ bool backward_slice(const Params& p, const Slice& sl,
           rg{region(st.g, ge * (int)sizeof(K)), st.g.pitch};
       const Rows<M> rs{region(st.st, (k - sl.first) * stat), st.st.pitch};
       auto rows_on = [](auto t, int r) { t.base += r * t.pitch; return t; };
-#define CUEQ_ROWS(D, N, R)                                                                                                             \
-  for (int r = 0; r < n; r += R)                                                                                                       \
-    backward_short<T, M, K, MODE, Q8, D, MUL_IR, N, R>(c, n - r, rows_on(ra, r), rows_on(rb, r), rows_on(rh, r), rows_on(ry, r), rows_on(rg, r), \
-                                                       rows_on(rd, r), rows_on(rs, r), has_go);
-#define CUEQ_SHORT(D, N)                                                                                                               \
-  if constexpr (kRowsAtOnce<D, N> > 1) {                                                                                               \
-    if (n > 1) { CUEQ_ROWS(D, N, (kRowsAtOnce<D, N>)) } else { CUEQ_ROWS(D, N, 1) }                                                    \
-  } else { CUEQ_ROWS(D, N, 1) }
+#define CUEQ_ROWS(D, N, R, NARROW, STEP)                                                                                                \
+  for (int r = 0; r < n; r += STEP)                                                                                                    \
+    backward_short<T, M, K, MODE, Q8, D, MUL_IR, N, R, NARROW>(c, n - r, rows_on(ra, r), rows_on(rb, r), rows_on(rh, r), rows_on(ry, r), \
+                                                               rows_on(rg, r), rows_on(rd, r), rows_on(rs, r), has_go);
 #define CUEQ_LONG(D)                                                                                                                   \
   for (int r = 0; r < n; ++r) backward_item<T, M, K, MODE, Q8, D, MUL_IR>(c, ra[r], rb[r], rh[r], ry[r], rg[r], rd[r], rs[r], has_go);
       CUEQ_NORM_DIMS(CUEQ_SHORT, CUEQ_LONG)
 #undef CUEQ_LONG
-#undef CUEQ_SHORT
 #undef CUEQ_ROWS
     }
   });
   // this warp's sums of the parameters' gradients
   M* dst = reinterpret_cast<M*>(p.parts) + (int64_t)blockIdx.x * p.channels + b0.ch;
-  for (int u = threadIdx.x; u < sl.channels; u += 32) {
-    if (MODE & kBranch) dst[u] = at[3 * sl.channels + u];
-    if (MODE & kNorm) dst[(int64_t)gridDim.x * p.channels + u] = at[4 * sl.channels + u];
+  for (int k = sl.first; k < sl.first + sl.count; ++k) {
+    const Blk& b = p.blk[k];
+    const M* sums = at + 3 * pad4(sl.channels) + b.sum;
+    const int groups = b.per_lane == 1 ? 32 / b.lanes : 1;
+    for (int u = threadIdx.x; u < b.mul; u += 32) {
+      M vs = M(0), vw = M(0);
+      for (int g = 0; g < groups; ++g) { vs += sums[g * b.lanes + u]; vw += sums[sl.sums + g * b.lanes + u]; }
+      if (MODE & kBranch) dst[b.ch - b0.ch + u] = vs;
+      if (MODE & kNorm) dst[(int64_t)gridDim.x * p.channels + b.ch - b0.ch + u] = vw;
+    }
   }
   __syncwarp();
   return done;

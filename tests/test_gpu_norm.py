@@ -84,7 +84,8 @@ def _residual(irreps, rows, dtype, layout, gate, norm_output, saved="full", seed
 SHAPES = [
     (L3, 1), (L3, 37), (L3, 2003),
     ("1x0e", 5), ("1x0e+1x1o+1x2e", 9), ("5x0e+3x1o+2x2e", 301), ("33x0e+7x1o", 64),
-    ("32x0e+32x1o+32x2e+32x3o", 1511), ("64x0e+64x1o", 4099), ("64x0e+32x0o+32x1o", 6), ("96x0e+64x2e+32x3o", 131), ("129x0e+97x1o", 47), ("96x0o+48x1e+16x2e+4x4e", 333),
+    ("32x0e+32x1o+32x2e+32x3o", 1511), ("64x0e+64x1o", 4099), ("64x0e+32x0o+32x1o", 6), ("96x0e+64x2e+32x3o", 131), ("129x0e+97x1o", 47),
+    ("2x0e+8x1o+16x2e+12x3o", 203), ("48x0e+36x1o+68x2e+100x3o", 77), ("3x0e+64x1o+128x2e", 41), ("20x0e+24x1o", 2), ("66x0e+34x1o", 35), ("96x0o+48x1e+16x2e+4x4e", 333),
     ("300x0e+260x3o", 55), ("2048x0e", 70), ("16x0e+16x0o+16x1e+16x1o+8x5o", 129),
 ]
 
