@@ -155,6 +155,7 @@ int make_plan(const cueq_norm_args* a, bool backward, bool dense, Params* p, int
   occupancy = occupancy < 1 ? 1 : occupancy > warps_per_sm(msize) ? warps_per_sm(msize) : occupancy;
   const int64_t units = (a->rows + unit - 1) / unit * ns, warps = (int64_t)kSms * occupancy;
   *grid = (int)(units < warps ? units : warps);
+  if (*grid) { p->deal = units / *grid; p->deal_more = (int)(units % *grid); }
   return 0;
 }
 
@@ -179,11 +180,11 @@ struct SumParams {
   void* out[2];
   int warps, channels, dtype;
 };
-constexpr int kSumRows = 32;
+constexpr int kSumRows = 128, kSumChannels = 8;   // eight channels, a sector of a warp's sums; 1,800 warps in 14 steps (32 x 32 threads: 50 steps, 8 us)
 template <class M>
-__global__ void __launch_bounds__(32 * kSumRows) sum_kernel(const __grid_constant__ SumParams p) {
-  __shared__ M partial[kSumRows][33];
-  const int ch = blockIdx.x * 32 + threadIdx.x;
+__global__ void __launch_bounds__(kSumChannels * kSumRows) sum_kernel(const __grid_constant__ SumParams p) {
+  __shared__ M partial[kSumRows][kSumChannels + 1];
+  const int ch = blockIdx.x * kSumChannels + threadIdx.x;
   const int which = blockIdx.y;
   M v = M(0);
   if (ch < p.channels && p.out[which]) {
@@ -193,10 +194,15 @@ __global__ void __launch_bounds__(32 * kSumRows) sum_kernel(const __grid_constan
   }
   partial[threadIdx.y][threadIdx.x] = v;
   __syncthreads();
+#pragma unroll
+  for (int n = kSumRows / 2; n >= 4; n /= 2) {
+    if (threadIdx.y < n) partial[threadIdx.y][threadIdx.x] += partial[threadIdx.y + n][threadIdx.x];
+    __syncthreads();
+  }
   if (threadIdx.y || ch >= p.channels || !p.out[which]) return;
   v = M(0);
 #pragma unroll
-  for (int j = 0; j < kSumRows; ++j) v += partial[j][threadIdx.x];
+  for (int j = 0; j < 4; ++j) v += partial[j][threadIdx.x];
   switch (p.dtype) {
     case CUEQ_F32: reinterpret_cast<float*>(p.out[which])[ch] = (float)v; break;
     case CUEQ_F64: reinterpret_cast<double*>(p.out[which])[ch] = (double)v; break;
@@ -262,7 +268,7 @@ int launch(const cueq_norm_args* a, bool backward, void* stream) {
   if (!backward) return 0;
   SumParams s{a->parts, {branch ? a->dscale : nullptr, norm ? a->dweight : nullptr}, a->rows ? grid : 0, p.channels, a->param_dtype};
   if (!s.out[0] && !s.out[1]) return 0;
-  const dim3 g((p.channels + 31) / 32, 2), t(32, kSumRows);
+  const dim3 g((p.channels + kSumChannels - 1) / kSumChannels, 2), t(kSumChannels, kSumRows);
   if (a->dtype == CUEQ_F64) sum_kernel<double><<<g, t, 0, st>>>(s);
   else sum_kernel<float><<<g, t, 0, st>>>(s);
   CUEQ_CUDA_OK(cudaGetLastError());

@@ -71,6 +71,8 @@ struct Params {
   double eps;
   int* status;
   int nb, ns, dim_total, channels;   // ns: statistics per (row, block)
+  int64_t deal;                      // units of rows and slices per warp; the first `deal_more` warps have one more
+  int deal_more;
   int num_slices, unit, stages;      // unit: rows after which dense rows are on a 16-byte boundary again; stages: 2, or 1 where two do not fit into shared memory
   int pdtype, gate, mul_ir;
   signed char route[kTensors];
@@ -784,14 +786,27 @@ __device__ __forceinline__ bool run_stages(const Params& p, int rps, int64_t fir
   return true;
 }
 
-// The rows of slice s for this warp.  Units of rows are dealt out row by row, all slices of one before the next, in equal numbers: every
+// The units of rows that this warp takes of each slice.  They are dealt out row by row, all slices of one before the next, in equal numbers: every
 // warp has its share of every slice, whatever a slice costs.
-__device__ __forceinline__ void my_rows(const Params& p, int s, int64_t& first, int64_t& last) {
-  const int64_t total = (p.rows + p.unit - 1) / p.unit * p.num_slices;
-  const int64_t a = total * blockIdx.x / gridDim.x, b = total * (blockIdx.x + 1) / gridDim.x;
-  first = (a - s + p.num_slices - 1) / p.num_slices * p.unit;
-  last = min(p.rows, (b - s + p.num_slices - 1) / p.num_slices * p.unit);
-}
+struct Share {
+  int64_t a, b;                      // units of the first slice; of slice s one more where s lies before `ra`, `rb`
+  int ra, rb;
+  __device__ __forceinline__ explicit Share(const Params& p) {
+    const int64_t j = blockIdx.x, from = j * p.deal + min(j, (int64_t)p.deal_more), to = from + p.deal + (j < p.deal_more ? 1 : 0);
+    a = divide(from, p.num_slices, ra);
+    b = divide(to, p.num_slices, rb);
+  }
+  static __device__ __forceinline__ int64_t divide(int64_t v, int n, int& rest) {
+    if (n == 1) { rest = 0; return v; }
+    const int64_t q = v < 0x7fffffff ? (int64_t)((unsigned)v / (unsigned)n) : v / n;
+    rest = (int)(v - q * n);
+    return q;
+  }
+  __device__ __forceinline__ void rows(const Params& p, int s, int64_t& first, int64_t& last) const {
+    first = (a + (s < ra)) * p.unit;
+    last = min(p.rows, (b + (s < rb)) * p.unit);
+  }
+};
 __device__ __forceinline__ void init_barriers(unsigned char* smem) {
   if (threadIdx.x == 0) {
     bar_init(reinterpret_cast<unsigned long long*>(smem), 1);
@@ -992,10 +1007,11 @@ __global__ void __launch_bounds__(32, warps_per_sm(sizeof(M))) forward_kernel(co
   extern __shared__ __align__(128) unsigned char smem[];
   init_barriers(smem);
   unsigned phases = 0;
-  for (int k = 0; k < p.num_slices; ++k) {               // neighbouring warps start with different slices
-    const int s = (k + blockIdx.x) % p.num_slices;
+  const Share share(p);
+  int s = blockIdx.x % p.num_slices;                     // neighbouring warps start with different slices
+  for (int k = 0; k < p.num_slices; ++k, s = s + 1 == p.num_slices ? 0 : s + 1) {
     int64_t first, last;
-    my_rows(p, s, first, last);
+    share.rows(p, s, first, last);
     if (first < last && !forward_slice<T, M, MODE, Q8, MUL_IR>(p, p.slice[s], first, last, smem, phases)) return;
   }
 }
@@ -1004,11 +1020,19 @@ __global__ void __launch_bounds__(32, warps_per_sm(sizeof(M))) backward_kernel(c
   extern __shared__ __align__(128) unsigned char smem[];
   init_barriers(smem);
   unsigned phases = 0;
-  for (int k = 0; k < p.num_slices; ++k) {
-    const int s = (k + blockIdx.x) % p.num_slices;
+  const Share share(p);
+  int s = blockIdx.x % p.num_slices;
+  for (int k = 0; k < p.num_slices; ++k, s = s + 1 == p.num_slices ? 0 : s + 1) {
     int64_t first, last;
-    my_rows(p, s, first, last);
-    if (!backward_slice<T, M, MODE, Q8, MUL_IR>(p, p.slice[s], first, last, smem, phases)) return;
+    share.rows(p, s, first, last);
+    if (first >= last) {                                 // fewer rows than warps: its sums are nothing
+      const Slice& sl = p.slice[s];
+      M* dst = reinterpret_cast<M*>(p.parts) + (int64_t)blockIdx.x * p.channels + p.blk[sl.first].ch;
+      for (int u = threadIdx.x; u < sl.channels; u += 32) {
+        if (MODE & kBranch) dst[u] = M(0);
+        if (MODE & kNorm) dst[(int64_t)gridDim.x * p.channels + u] = M(0);
+      }
+    } else if (!backward_slice<T, M, MODE, Q8, MUL_IR>(p, p.slice[s], first, last, smem, phases)) return;
   }
 }
 
