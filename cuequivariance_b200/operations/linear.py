@@ -187,26 +187,30 @@ class _FusedLinear(torch.autograd.Function):
 
         from .. import profiling
 
-        a = _lib.LinearArgs()
+        kept = plan.setdefault("arguments", {})           # what does not change from call to call
+        key = (which, transposed, len(bounds))
+        if key not in kept:
+            a = _lib.LinearArgs()
+            a.num_paths, a.num_classes = len(plan["paths"]), len(bounds) - 1
+            a.x_mul_ir, a.out_mul_ir = plan["mul_ir"] if not transposed else plan["mul_ir"][::-1]
+            a.transposed, a.struct_bytes = transposed, C.sizeof(a)
+            for q, (wo, u, v, xo, oo, d, c) in zip(a.paths, plan["paths"]):
+                q.u, q.v, q.d, q.x_off, q.out_off, q.w_off, q.c = u, v, d, xo, oo, wo, c
+            kept[key] = bytes(a)
+        a = _lib.LinearArgs.from_buffer_copy(kept[key])
         a.x, a.w, a.out = x.data_ptr(), w.data_ptr(), out.data_ptr()
-        a.bounds = _lib.int32_array(bounds)
-        a.status = _lib.status_word(x.device).data_ptr()
-        a.num_paths, a.num_classes = len(plan["paths"]), len(bounds) - 1
-        a.x_mul_ir, a.out_mul_ir = plan["mul_ir"] if not transposed else plan["mul_ir"][::-1]
-        a.transposed, a.struct_bytes = transposed, C.sizeof(a)
+        held = _lib.int32_array(bounds)
+        a.bounds, a.status = held, _lib.status_word(x.device).data_ptr()
         a.ldx, a.ldo = plan["in_size"] if codes is not None else x.shape[1], (out if which == "map" else w).shape[1]
         a.w_class_stride = (w if which == "map" else out).shape[1]
-        for q, (wo, u, v, xo, oo, d, c) in zip(a.paths, plan["paths"]):
-            q.u, q.v, q.d, q.x_off, q.out_off, q.w_off, q.c = u, v, d, xo, oo, wo, c
         L = _lib.lib()
-        stream = C.c_void_p(torch.cuda.current_stream(x.device).cuda_stream)
+        c = None
         if codes is not None:
             values, steps = codes
             c = _lib.LinearCodes()
             c.struct_bytes, c.rows = C.sizeof(c), values.shape[0]
             c.codes, c.ld_codes, c.steps, c.ld_steps = values.data_ptr(), values.shape[1], steps.data_ptr(), steps.shape[1]
-            gw_codes = L.cueq_b200_linear_pack if which == "pack" else L.cueq_b200_linear_gw_codes
-            fn = lambda args, stream: gw_codes(args, C.byref(c), stream)  # noqa: E731
+            fn = L.cueq_b200_linear_pack if which == "pack" else L.cueq_b200_linear_gw_codes
         else:
             fn = L.cueq_b200_linear_map if which == "map" else L.cueq_b200_linear_gw
         parts = None
@@ -215,8 +219,9 @@ class _FusedLinear(torch.autograd.Function):
             parts = torch.empty(max(n, 0), dtype=torch.float32, device=x.device)
             a.parts, a.parts_floats = parts.data_ptr(), n
         name = ("linear" if len(bounds) == 2 else "indexed_linear") + "_f32x3" + ("_gx" if transposed else "" if which == "map" else f"_{which}")
-        with torch.cuda.device(x.device), profiling.kernel(name):
-            _lib.check(fn(C.byref(a), stream))
+        with _lib.on_device(x.device), profiling.kernel(name):
+            stream = torch._C._cuda_getCurrentRawStream(x.device.index)
+            _lib.check(fn(C.byref(a), stream) if c is None else fn(C.byref(a), C.byref(c), stream))
 
     @staticmethod
     def _apply(plan, bounds, weight, x):

@@ -20,6 +20,7 @@ from .. import _lib, profiling
 from ..executor import dtype_code
 from ..irreps import Irreps, IrrepsLayout
 
+_NAMES = {_lib.NORM_BRANCH: "gated_residual_", _lib.NORM_ALONE: "irreps_norm_", _lib.NORM_BOTH: "gated_residual_norm_"}
 SAVED_ACTIVATIONS = ("full", "int8")
 _TYPES = (torch.float32, torch.float64, torch.bfloat16, torch.float16)
 
@@ -108,15 +109,8 @@ class _Block:
     def launch(self, which: str, a: "_lib.NormArgs", device: torch.device) -> None:
         L = _lib.lib()
         fn = L.cueq_b200_norm_forward if which == "forward" else L.cueq_b200_norm_backward
-        with _lib.on_device(device):
-            stream = torch._C._cuda_getCurrentRawStream(device.index)
-            if not profiling.enabled():
-                profiling.launch_count += 1
-                _lib.check(fn(C.byref(a), stream))
-                return
-            name = {_lib.NORM_BRANCH: "gated_residual", _lib.NORM_ALONE: "irreps_norm", _lib.NORM_BOTH: "gated_residual_norm"}[a.mode]
-            with profiling.kernel(f"{name}_{which}"):
-                _lib.check(fn(C.byref(a), stream))
+        with _lib.on_device(device), profiling.kernel(_NAMES[a.mode] + which):
+            _lib.check(fn(C.byref(a), torch._C._cuda_getCurrentRawStream(device.index)))
 
     def forward(self, keep: bool, x, y, g, s, w):
         """(out, norm, codes, stats) - the last two for a backward pass to come."""

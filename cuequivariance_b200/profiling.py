@@ -29,14 +29,28 @@ def reset() -> None:
     launch_count = 0
 
 
-@contextlib.contextmanager
+class _Uncounted:
+    """What ``kernel`` returns while timing is off: a generator's context manager costs 1.5 us a launch."""
+
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        pass
+
+
+_uncounted = _Uncounted()
+
+
 def kernel(name: str, stream=None):
     """Brackets one native launch."""
     global launch_count
     launch_count += 1
-    if not _enabled:
-        yield
-        return
+    return _timed(name) if _enabled else _uncounted
+
+
+@contextlib.contextmanager
+def _timed(name: str):
     import torch
 
     s, e = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
