@@ -8,7 +8,7 @@ namespace {
 
 using namespace cueq_norm;
 
-constexpr int kSmemPerSm = 227 * 1024, kSms = 148;
+constexpr int kSmemPerSm = 227 * 1024;
 constexpr int kSliceValues = 1024;       // neighbouring irrep blocks are put together up to this length
 constexpr int kStageBytes = 4096;        // rows are put together up to about this much per stage
 
