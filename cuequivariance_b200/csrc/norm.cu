@@ -10,6 +10,7 @@ using namespace cueq_norm;
 
 constexpr int kSmemPerSm = 227 * 1024;
 constexpr int kSliceValues = 1024;       // neighbouring irrep blocks are put together up to this length
+constexpr int kWarpsOfLongBlocks = 9;
 constexpr int kStageBytes = 4096;        // rows are put together up to about this much per stage
 
 int element_size(int dtype) { return dtype == CUEQ_F64 ? 8 : dtype == CUEQ_F32 ? 4 : 2; }
@@ -104,7 +105,7 @@ int make_plan(const cueq_norm_args* a, bool backward, bool dense, Params* p, int
     b.mul = a->blocks[k].mul; b.dim = (short)a->blocks[k].dim;
     b.off = p->dim_total; b.ch = p->channels;
     const int n = b.mul * b.dim;
-    if (!ns || p->slice[ns - 1].values + n > kSliceValues) { p->slice[ns] = Slice{}; p->slice[ns].first = k; ++ns; }
+    if (!ns || p->slice[ns - 1].values + n > kSliceValues) { p->slice[ns] = Slice{}; p->slice[ns].first = (short)k; ++ns; }
     Slice& s = p->slice[ns - 1];
     if (s.count == 0 && (b.off * size % 16 || (gated(a) && b.ch * size % 16))) even = false;
     ++s.count; s.values += n; s.channels += b.mul;
@@ -116,7 +117,7 @@ int make_plan(const cueq_norm_args* a, bool backward, bool dense, Params* p, int
   int unit = 1;                                          // rows after which dense rows are on a 16-byte boundary again
   if (dense && ns == 1) while (unit < 8 && (unit * p->dim_total * size % 16 || (gated(a) && unit * p->channels * size % 16))) unit *= 2;
   auto stage = [&](const Slice& s) { return backward ? backward_stage(*p, s, a->mode, q8, size, stat).total : forward_stage(*p, s, a->mode, q8, size).total; };
-  auto need = [&](const Slice& s, int stages) { return head_bytes(msize, s, backward) + stages * stage(s); };
+  auto need = [&](const Slice& s, int stages) { return head_bytes(msize, s, a->mode, backward) + stages * stage(s); };
   // How a block is worked on: up to 32, 64 or 128 channels by 1, 2 or 4 per lane, where these are neighbours on a boundary of as many
   // values in every row; up to 16 channels with several rows side by side.  The rest, l > 3 among it, goes through loops (256 channels: 0.6
   // of the copy bandwidth where 128 have 0.75).
@@ -132,6 +133,7 @@ int make_plan(const cueq_norm_args* a, bool backward, bool dense, Params* p, int
       while (b.per_lane == 1 && b.lanes / 2 >= b.mul) b.lanes /= 2;
       b.sum = s.sums;
       s.sums += pad4(b.lanes < 32 ? 32 : b.mul);
+      if (!b.per_lane) s.loops = 1;
     }
   }
   p->stages = 2;
@@ -139,13 +141,15 @@ int make_plan(const cueq_norm_args* a, bool backward, bool dense, Params* p, int
   int smem = 0;
   for (int k = 0; k < ns; ++k) {
     Slice& s = p->slice[k];
-    s.rps = unit;
+    s.rps = (short)unit;
     if (unit > 1 && need(s, 2) > kSmemPerSm / 2) return kTooLongForUnits;
     if (need(s, 2) > kSmemPerSm) p->stages = 1;
     const int one = stage(s) / unit;
-    int rps = kStageBytes / (one ? one : 1) / unit * unit;
+    int rps = kStageBytes / (one ? one : 1) / unit * unit, beside = 1;
+    for (int k2 = s.first; k2 < s.first + s.count; ++k2) beside = 32 / p->blk[k2].lanes > beside ? 32 / p->blk[k2].lanes : beside;
+    while (rps < beside && (rps + unit) * one <= 2 * kStageBytes) rps += unit;   // rows that a warp takes side by side
     rps = rps >= 3 ? (rps + 1) / 4 * 4 : rps;            // rows are worked on by fours, twos or one by one
-    s.rps = rps < unit ? unit : rps > 32 ? 32 : rps;
+    s.rps = (short)(rps < unit ? unit : rps > 32 ? 32 : rps);
     while (s.rps > unit && copy_lanes(a, backward, *p, s.rps) > 32) s.rps -= unit;
   }
   for (int k = 0; k < ns; ++k) { const int b = need(p->slice[k], p->stages); smem = b > smem ? b : smem; }
@@ -153,6 +157,10 @@ int make_plan(const cueq_norm_args* a, bool backward, bool dense, Params* p, int
   if (smem > kSmemPerSm) return kTooLong;
   int occupancy = kSmemPerSm / (smem + 1024);
   occupancy = occupancy < 1 ? 1 : occupancy > warps_per_sm(msize) ? warps_per_sm(msize) : occupancy;
+  // Long blocks in full are bound by HBM, which serves 9 warps per SM with 60 KB under way better than 14 (32,768 rows of 128x(0e+1o+2e+3o) in
+  // float32: norm 155 and 168 us backward, gated residual 155 and 164 us forward); the others are bound by instructions and want all
+  // (64x0e, gated residual: 123 us, with 8 warps 167 us).
+  if (a->mode != kBoth && !q8 && size >= 4 && p->dim_total / a->num_blocks >= 384 && occupancy > kWarpsOfLongBlocks) occupancy = kWarpsOfLongBlocks;
   const int64_t units = (a->rows + unit - 1) / unit * ns, warps = (int64_t)kSms * occupancy;
   *grid = (int)(units < warps ? units : warps);
   if (*grid) { p->deal = units / *grid; p->deal_more = (int)(units % *grid); }

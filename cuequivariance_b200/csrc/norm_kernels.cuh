@@ -48,10 +48,11 @@ struct Blk {
   unsigned char per_lane, lanes;     // neighbouring channels of a lane (0: any number, one by one), lanes of a row
 };
 struct Slice {
-  int first, count;                  // blocks
-  int values, channels;              // their elements and channels
+  short first, count;                // blocks
+  short rps;                         // rows per stage
+  short loops;                       // some block has more channels than registers hold
+  int values, channels;              // of its blocks
   int sums;                          // sums per parameter: one per channel, or per channel of every row that a warp takes at a time
-  int rps;                           // rows per stage
 };
 // How rows of an operand move.  kRows: a bulk copy per row; kDense: rows follow one another without a gap, one bulk copy per stage;
 // kPlain: element by element, where addresses or lengths are not multiples of 16 bytes.
@@ -139,10 +140,23 @@ __host__ __device__ inline Stage backward_stage(const Params& p, const Slice& s,
   t.total = at;
   return t;
 }
-// in front of the stages: 2 barriers and the tensors' moves; per channel s, w, s act(g) of the row at work, and (backward) the sums of both gradients
+// in front of the stages: 2 barriers and the tensors' moves; then per channel, as far as the mode has them, s, w, s act(g) of the row at work (for
+// the loops), and (backward) the sums of both gradients
 constexpr int kMoves = 11, kMoveBytes = 40, kBars = 16 + kMoves * kMoveBytes + 8;
 __host__ __device__ constexpr int pad4(int n) { return (n + 3) & ~3; }
-__host__ __device__ inline int head_bytes(int msize, const Slice& s, bool backward) { return (kBars + msize * (3 * pad4(s.channels) + (backward ? 2 * s.sums : 0)) + 127) & ~127; }
+struct Head { int s, w, a, sum_s, sum_w, total; };
+__host__ __device__ inline Head head_of(const Slice& s, int mode, bool backward) {
+  const int n = pad4(s.channels);
+  Head h;
+  h.s = 0;
+  h.w = h.s + (mode & kBranch ? n : 0);
+  h.a = h.w + (mode & kNorm ? n : 0);
+  h.sum_s = h.a + ((mode & kBranch) && s.loops ? n : 0);
+  h.sum_w = h.sum_s + (backward && (mode & kBranch) ? s.sums : 0);
+  h.total = h.sum_w + (backward && (mode & kNorm) ? s.sums : 0);
+  return h;
+}
+__host__ __device__ inline int head_bytes(int msize, const Slice& s, int mode, bool backward) { return (kBars + msize * head_of(s, mode, backward).total + 127) & ~127; }
 
 // ---- conversions ----------------------------------------------------------------------------------------------------
 template <class M> __device__ __forceinline__ M to(float v) { return (M)v; }
@@ -818,22 +832,23 @@ __device__ __forceinline__ void init_barriers(unsigned char* smem) {
   __syncwarp();
 }
 // parameters of the slice's channels into shared memory, sums cleared
-template <class M>
-__device__ __forceinline__ void prepare(const Params& p, const Slice& s, M* at, bool backward) {
-  const int ch = p.blk[s.first].ch, n = pad4(s.channels);
+template <class M, int MODE, bool BACKWARD>
+__device__ __forceinline__ void prepare(const Params& p, const Slice& s, M* at) {
+  const int ch = p.blk[s.first].ch;
+  const Head h = head_of(s, MODE, BACKWARD);
   for (int u = threadIdx.x; u < s.channels; u += 32) {
-    at[u] = p.s ? cueq::load_as<M>(p.s, p.pdtype, ch + u) : M(1);
-    at[n + u] = p.w ? cueq::load_as<M>(p.w, p.pdtype, ch + u) : M(1);
+    if (MODE & kBranch) at[h.s + u] = cueq::load_as<M>(p.s, p.pdtype, ch + u);
+    if (MODE & kNorm) at[h.w + u] = cueq::load_as<M>(p.w, p.pdtype, ch + u);
   }
-  if (backward)
-    for (int u = threadIdx.x; u < 2 * s.sums; u += 32) at[3 * n + u] = M(0);
+  for (int u = h.sum_s + threadIdx.x; u < h.total; u += 32) at[u] = M(0);
   __syncwarp();
 }
-template <class M>
+template <class M, int MODE, bool BACKWARD>
 __device__ __forceinline__ View<M> block_view(const Params& p, const Slice& s, const Blk& b, M* at) {
   View<M> c;
-  const int u0 = b.ch - p.blk[s.first].ch, n = pad4(s.channels);
-  c.s = at + u0; c.w = at + n + u0; c.a = at + 2 * n + u0; c.acc_s = at + 3 * n + b.sum; c.acc_w = c.acc_s + s.sums;
+  const int u0 = b.ch - p.blk[s.first].ch;
+  const Head h = head_of(s, MODE, BACKWARD);
+  c.s = at + h.s + u0; c.w = at + h.w + u0; c.a = at + h.a + u0; c.acc_s = at + h.sum_s + b.sum; c.acc_w = at + h.sum_w + b.sum;
   c.mul = b.mul; c.dim = b.dim;
   c.lane = threadIdx.x; c.lanes = b.lanes;
   c.gate = p.gate; c.gated = p.gate != CUEQ_NORM_GATE_NONE;
@@ -904,11 +919,11 @@ __device__ __forceinline__ bool forward_slice(const Params& p, const Slice& sl, 
   const int nout = 1 + (MODE == kBoth) + (Q8 ? 1 + (MODE == kBoth) + gated : 0);
   const int nin = (MODE & kBranch) ? 2 + gated : 1;
   put_moves(moves, in, nin, out, nout);
-  return run_stages(p, sl.rps, first, last, moves, nin, moves + nin, nout, smem + head_bytes(sizeof(M), sl, false), st.total,
-                    reinterpret_cast<unsigned long long*>(smem), phases, [&]() { prepare<M>(p, sl, at, false); }, [&](unsigned char* s, int64_t z, int n) {
+  return run_stages(p, sl.rps, first, last, moves, nin, moves + nin, nout, smem + head_bytes(sizeof(M), sl, MODE, false), st.total,
+                    reinterpret_cast<unsigned long long*>(smem), phases, [&]() { prepare<M, MODE, false>(p, sl, at); }, [&](unsigned char* s, int64_t z, int n) {
     for (int k = sl.first; k < sl.first + sl.count; ++k) {
       const Blk& b = p.blk[k];
-      const View<M> c = block_view<M>(p, sl, b, at);
+      const View<M> c = block_view<M, MODE, false>(p, sl, b, at);
       const int e = b.off - b0.off, u = b.ch - b0.ch;
       auto region = [&](const Region& reg, int bytes) { return s + reg.at + bytes; };
       const Rows<T> rx{region(st.a, e * size), st.a.pitch}, ry{region(st.b, e * size), st.b.pitch}, rg{region(st.g, u * size), st.g.pitch};
@@ -963,11 +978,11 @@ __device__ __forceinline__ bool backward_slice(const Params& p, const Slice& sl,
   const Move out[3] = {MODE == kNorm ? o_b : o_a, MODE == kBoth ? o_b : o_g, o_g};
   const int nout = MODE == kNorm ? 1 : 1 + (MODE == kBoth) + gated;
   put_moves(moves, in, nin, out, nout);
-  const bool done = run_stages(p, sl.rps, first, last, moves, nin, moves + nin, nout, smem + head_bytes(sizeof(M), sl, true), st.total,
-                               reinterpret_cast<unsigned long long*>(smem), phases, [&]() { prepare<M>(p, sl, at, true); }, [&](unsigned char* s, int64_t, int n) {
+  const bool done = run_stages(p, sl.rps, first, last, moves, nin, moves + nin, nout, smem + head_bytes(sizeof(M), sl, MODE, true), st.total,
+                               reinterpret_cast<unsigned long long*>(smem), phases, [&]() { prepare<M, MODE, true>(p, sl, at); }, [&](unsigned char* s, int64_t, int n) {
     for (int k = sl.first; k < sl.first + sl.count; ++k) {
       const Blk& b = p.blk[k];
-      const View<M> c = block_view<M>(p, sl, b, at);
+      const View<M> c = block_view<M, MODE, true>(p, sl, b, at);
       const int e = b.off - b0.off, u = b.ch - b0.ch;
       const int ce = Q8 ? b.code - b0.code : e, he = Q8 ? (MODE == kBoth ? b.hcode - b0.hcode : b.code - b0.code) : e, ge = Q8 ? b.gcode - b0.gcode : u;
       auto region = [&](const Region& reg, int bytes) { return s + reg.at + bytes; };
@@ -989,13 +1004,17 @@ __device__ __forceinline__ bool backward_slice(const Params& p, const Slice& sl,
   });
   // this warp's sums of the parameters' gradients
   M* dst = reinterpret_cast<M*>(p.parts) + (int64_t)blockIdx.x * p.channels + b0.ch;
+  const Head head = head_of(sl, MODE, true);
   for (int k = sl.first; k < sl.first + sl.count; ++k) {
     const Blk& b = p.blk[k];
-    const M* sums = at + 3 * pad4(sl.channels) + b.sum;
+    const M *sums_s = at + head.sum_s + b.sum, *sums_w = at + head.sum_w + b.sum;
     const int groups = b.per_lane == 1 ? 32 / b.lanes : 1;
     for (int u = threadIdx.x; u < b.mul; u += 32) {
       M vs = M(0), vw = M(0);
-      for (int g = 0; g < groups; ++g) { vs += sums[g * b.lanes + u]; vw += sums[sl.sums + g * b.lanes + u]; }
+      for (int g = 0; g < groups; ++g) {
+        if (MODE & kBranch) vs += sums_s[g * b.lanes + u];
+        if (MODE & kNorm) vw += sums_w[g * b.lanes + u];
+      }
       if (MODE & kBranch) dst[b.ch - b0.ch + u] = vs;
       if (MODE & kNorm) dst[(int64_t)gridDim.x * p.channels + b.ch - b0.ch + u] = vw;
     }

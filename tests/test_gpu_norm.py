@@ -224,6 +224,20 @@ def test_gradients_against_differences():
             assert abs((up - down) / 2e-6 - got) <= 1e-6 * (1 + abs(got)), names[k]
 
 
+@pytest.mark.parametrize("irreps", ["7000x0e", "1200x0e+3000x1o+33x0o"])
+def test_blocks_that_leave_room_for_one_stage(irreps):
+    for layout in (cb.mul_ir, cb.ir_mul):
+        _norm(irreps, 5, F32, layout)
+        _residual(irreps, 5, BF16, layout, "sigmoid", True)
+        _residual(irreps, 3, F32, layout, None, False, "int8")
+
+
+def test_blocks_that_do_not_fit_are_refused():
+    m = cb.GatedResidual("30000x0e", gate=None)
+    with pytest.raises(RuntimeError, match="shared memory"):
+        m.to(DEV)(torch.zeros(2, 30000, device=DEV), torch.zeros(2, 30000, device=DEV))
+
+
 def test_second_derivatives_are_refused():
     m = cb.GatedResidual("32x0e+3x1o", norm_output=True).to(DEV)
     x, g = torch.randn(5, 41, device=DEV, requires_grad=True), torch.randn(5, 35, device=DEV)
