@@ -10,7 +10,7 @@ using namespace cueq_norm;
 
 constexpr int kSmemPerSm = 227 * 1024;
 constexpr int kSliceValues = 1024;       // neighbouring irrep blocks are put together up to this length
-constexpr int kWarpsOfLongBlocks = 9;
+constexpr int kWarpsOfLongBlocks = 9, kFewWarps = 7;
 constexpr int kStageBytes = 4096;        // rows are put together up to about this much per stage
 
 int element_size(int dtype) { return dtype == CUEQ_F64 ? 8 : dtype == CUEQ_F32 ? 4 : 2; }
@@ -27,7 +27,7 @@ int check(const cueq_norm_args* a) {
   if (a->num_blocks < 1 || a->num_blocks > kMaxBlocks || !a->blocks) return cueq::fail("norm: between 1 and %d irrep blocks", kMaxBlocks);
   if (a->rows < 0 || a->rows >= (int64_t(1) << 40)) return cueq::fail("norm: bad number of rows");
   for (int k = 0; k < a->num_blocks; ++k)
-    if (a->blocks[k].mul < 1 || a->blocks[k].dim < 1 || a->blocks[k].dim > 32767 || (int64_t)a->blocks[k].mul * a->blocks[k].dim > (1 << 24)) return cueq::fail("norm: bad irrep block %d", k);
+    if (a->blocks[k].mul < 1 || a->blocks[k].dim < 1 || a->blocks[k].dim > 32767 || (int64_t)a->blocks[k].mul * a->blocks[k].dim > (1 << 20)) return cueq::fail("norm: bad irrep block %d", k);
   if (a->stats_stride && a->stats_stride != 8 && (a->stats_stride != 4 || (a->codes && a->mode == kBoth))) return cueq::fail("norm: bad stride of the statistics");
   if (!(a->eps > 0)) return cueq::fail("norm: eps must be positive");
   if (a->codes && a->dtype == CUEQ_F64) return cueq::fail("norm: 64-bit data are not kept in 8 bits");
@@ -136,14 +136,12 @@ int make_plan(const cueq_norm_args* a, bool backward, bool dense, Params* p, int
       if (!b.per_lane) s.loops = 1;
     }
   }
-  p->stages = 2;
   p->unit = unit;
   int smem = 0;
   for (int k = 0; k < ns; ++k) {
     Slice& s = p->slice[k];
     s.rps = (short)unit;
     if (unit > 1 && need(s, 2) > kSmemPerSm / 2) return kTooLongForUnits;
-    if (need(s, 2) > kSmemPerSm) p->stages = 1;
     const int one = stage(s) / unit;
     int rps = kStageBytes / (one ? one : 1) / unit * unit, beside = 1;
     for (int k2 = s.first; k2 < s.first + s.count; ++k2) beside = 32 / p->blk[k2].lanes > beside ? 32 / p->blk[k2].lanes : beside;
@@ -152,11 +150,19 @@ int make_plan(const cueq_norm_args* a, bool backward, bool dense, Params* p, int
     s.rps = (short)(rps < unit ? unit : rps > 32 ? 32 : rps);
     while (s.rps > unit && copy_lanes(a, backward, *p, s.rps) > 32) s.rps -= unit;
   }
-  for (int k = 0; k < ns; ++k) { const int b = need(p->slice[k], p->stages); smem = b > smem ? b : smem; }
-  *smem_bytes = smem;
-  if (smem > kSmemPerSm) return kTooLong;
-  int occupancy = kSmemPerSm / (smem + 1024);
-  occupancy = occupancy < 1 ? 1 : occupancy > warps_per_sm(msize) ? warps_per_sm(msize) : occupancy;
+  auto fit = [&](int stages) {                           // warps per SM, 0: none
+    p->stages = stages;
+    smem = 0;
+    for (int k = 0; k < ns; ++k) { const int b = need(p->slice[k], stages); smem = b > smem ? b : smem; }
+    *smem_bytes = smem;
+    return smem > kSmemPerSm ? 0 : smem + 1024 > kSmemPerSm ? 1 : kSmemPerSm / (smem + 1024);
+  };
+  // Where two stages leave room for few warps, twice as many with one stage each are better (256x(0e+1o+2e+3o) with the next norm, backward:
+  // 348 us with four warps, 239 with eight).
+  int occupancy = fit(2);
+  if (occupancy < kFewWarps) occupancy = fit(1);
+  if (occupancy < 1) return kTooLong;
+  occupancy = occupancy > warps_per_sm(msize) ? warps_per_sm(msize) : occupancy;
   // Long blocks in full are bound by HBM, which serves 9 warps per SM with 60 KB under way better than 14 (32,768 rows of 128x(0e+1o+2e+3o) in
   // float32: norm 155 and 168 us backward, gated residual 155 and 164 us forward); the others are bound by instructions and want all
   // (64x0e, gated residual: 123 us, with 8 warps 167 us).

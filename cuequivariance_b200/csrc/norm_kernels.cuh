@@ -75,7 +75,7 @@ struct Params {
   int nb, ns, dim_total, channels;   // ns: statistics per (row, block)
   int64_t deal;                      // units of rows and slices per warp; the first `deal_more` warps have one more
   int deal_more;
-  int num_slices, unit, stages;      // unit: rows after which dense rows are on a 16-byte boundary again; stages: 2, or 1 where two do not fit into shared memory
+  int num_slices, unit, stages;      // unit: rows after which dense rows are on a 16-byte boundary again; stages: 2, or 1 where two leave room for few warps
   int pdtype, gate, mul_ir;
   signed char route[kTensors];
   Blk blk[kMaxBlocks];
@@ -746,7 +746,7 @@ __device__ __forceinline__ Job make_job(const Move* moves, int count, int rps, i
 __device__ __forceinline__ unsigned job_bytes(const Job& j, int n) { return j.row < 0 ? (unsigned)(n * j.bytes) & ~15u : j.row < n ? j.bytes : 0u; }
 
 // Rows first .. last in stages of rps rows; `work(stage, z, n)`.  A lane that issues loads into a stage waits for its own stores out of
-// it; the warp then meets, so that no lane's load overtakes another lane's store.  One stage at a time where two do not fit.
+// it; the warp then meets, so that no lane's load overtakes another lane's store.  Or one stage at a time.
 // `ready()` runs while the first loads are under way.  `phases`, bit s: the phase that stage s waits for.  False: given up.
 template <class Ready, class Work>
 __device__ __forceinline__ bool run_stages(const Params& p, int rps, int64_t first, int64_t last, const Move* in, int nin, const Move* out, int nout,
