@@ -11,12 +11,19 @@
 // (r c and no r^3: that leaves the range of 32 bits for blocks of 1e13 or 1e-13)
 // and the same with (w, gn, h) for (a, go, y) for the norm; behind a branch its result is added to go first.
 //
-// What bounds them: HBM.  Every value is read once and written once.  A thread block is one warp.  It belongs to a slice of the
-// irrep blocks (neighbours of 1,024 values together, one block if that is longer) and to a range of rows, and brings the slice's part of a few rows
-// into shared memory by bulk copies, the next stage while it works on this one: no barrier between warps anywhere, and 7 to 30 stages
-// under way per SM.  A lane owns channels and reads their components in shared memory at a stride of dim words (odd: no bank conflicts;
-// neighbouring words in ir_mul), so neither layout needs a transposition and sums over components need no other lane.  Results
-// replace the operands in shared memory and leave by bulk copies.
+// What bounds them: HBM, for long blocks in 32 bits; every value is read once and written once.  A thread block is one warp with memory of
+// its own, so that nothing waits for another warp.  It takes its share of rows of every slice (neighbouring irrep blocks of 1,024 values together, or
+// a longer one) and brings the slice's part of a few rows into shared memory by bulk copies, a copy per lane, the next stage while it works on
+// this one; 60 to 90 KB are under way per SM.  A lane owns neighbouring channels and all their components, so neither layout needs a
+// transposition and sums over components need no other lane; blocks of up to 128 channels are read from shared memory into registers once.
+// Results replace the operands in shared memory and leave by bulk copies.
+//
+// Steps, for 32,768 rows of 128x(0e+1o+2e+3o) in float32, forward + backward (HBM floor of the norm 82 + 123 us, of the gated residual
+// 133 + 143, with the next norm 174 + 266): four warps on an item 120 + 158, 231 + 315, 359 + 439; a warp per slice 106 + 175, 183 + 226,
+// 240 + 473; every warp on every slice 108 + 157, 156 + 178, 210 + 339; fewer warps for long blocks 100 + 146 (5.4 and 5.5 TB/s),
+// 152 + 171 (5.7 and 5.5 TB/s), 214 + 310 (5.3 and 5.6 TB/s).  Short blocks, 16-bit data and codes are bound by instructions: 262,144 rows of
+// 64x(0e+1o) in bfloat16 115 + 149 us (floor 72 + 82), 0.7 of the issue slots used; the gate's exponential and the sums over the warp
+// are most of them.
 //
 // Sums, statistics and all arithmetic are in 32 bits for 16- and 32-bit data, in 64 for 64-bit data; results are rounded once.
 //
@@ -57,7 +64,7 @@ struct Slice {
 // How rows of an operand move.  kRows: a bulk copy per row; kDense: rows follow one another without a gap, one bulk copy per stage;
 // kPlain: element by element, where addresses or lengths are not multiples of 16 bytes.
 enum Route { kPlain, kRows, kDense };
-enum Tensor { tX, tY, tG, tH, tGo, tGn, tOut, tNorm, tDx, tDy, tDg, tCa, tCg, tCh, tStats, kTensors };
+enum Tensor { tX, tY, tG, tH, tGo, tGn, tOut, tNorm, tDx, tDy, tDg, tStats, kTensors };
 
 struct Params {
   const void *x, *y, *g, *h, *go, *gn;
@@ -778,6 +785,7 @@ __device__ __forceinline__ bool run_stages(const Params& p, int rps, int64_t fir
     if (!__all_sync(0xffffffffu, bar_wait(full + s, phases >> s & 1, p.status))) {   // a copy did not arrive in time: give up once those in flight have landed
       if (two && more) bar_wait(full + (s ^ 1), phases >> (s ^ 1) & 1, p.status);
       bar_wait(full + s, phases >> s & 1, p.status);
+      asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
       return false;
     }
     phases ^= 1u << s;
