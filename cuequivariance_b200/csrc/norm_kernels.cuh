@@ -844,10 +844,26 @@ template <class M, int MODE, bool BACKWARD>
 __device__ __forceinline__ void prepare(const Params& p, const Slice& s, M* at) {
   const int ch = p.blk[s.first].ch;
   const Head h = head_of(s, MODE, BACKWARD);
-  for (int u = threadIdx.x; u < s.channels; u += 32) {
-    if (MODE & kBranch) at[h.s + u] = cueq::load_as<M>(p.s, p.pdtype, ch + u);
-    if (MODE & kNorm) at[h.w + u] = cueq::load_as<M>(p.w, p.pdtype, ch + u);
-  }
+  // 128 channels at a time: all loads before the first store
+  auto fill = [&](auto load) {
+    for (int u = threadIdx.x; u < s.channels; u += 128) {
+      M vs[4], vw[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int v = min(u + 32 * q, s.channels - 1);
+        if (MODE & kBranch) vs[q] = load(p.s, ch + v);
+        if (MODE & kNorm) vw[q] = load(p.w, ch + v);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (u + 32 * q < s.channels) {
+          if (MODE & kBranch) at[h.s + u + 32 * q] = vs[q];
+          if (MODE & kNorm) at[h.w + u + 32 * q] = vw[q];
+        }
+    }
+  };
+  if (p.pdtype == (sizeof(M) == 8 ? CUEQ_F64 : CUEQ_F32)) fill([](const void* q, int i) { return __ldg(reinterpret_cast<const M*>(q) + i); });
+  else fill([&](const void* q, int i) { return cueq::load_as<M>(q, p.pdtype, i); });
   for (int u = h.sum_s + threadIdx.x; u < h.total; u += 32) at[u] = M(0);
   __syncwarp();
 }
