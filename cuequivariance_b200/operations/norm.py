@@ -46,8 +46,8 @@ class _Block:
         muls = [(mul, ir.dim) for mul, ir in irreps if mul > 0]
         if not 1 <= len(muls) <= _lib.NORM_MAX_BLOCKS:
             raise ValueError(f"irreps of 1 to {_lib.NORM_MAX_BLOCKS} blocks are supported, got {irreps}")
-        if not eps > 0:
-            raise ValueError(f"eps must be positive, got {eps}")
+        if not 0 < eps < float("inf"):
+            raise ValueError(f"eps must be positive and finite, got {eps}")
         self.blocks = (_lib.NormBlock * len(muls))(*muls)
         self.dim, self.channels = sum(m * d for m, d in muls), sum(m for m, _ in muls)
         self.layout, self.eps, self.mode, self.gate, self.int8 = layout, eps, mode, gate, int8

@@ -11,7 +11,7 @@ from cuequivariance_b200 import _lib
 
 
 def test_constructor_refusals():
-    for bad in (dict(eps=0.0), dict(eps=-1.0), dict(eps=float("nan")), dict(saved_activations="int4")):
+    for bad in (dict(eps=0.0), dict(eps=-1.0), dict(eps=float("nan")), dict(eps=float("inf")), dict(saved_activations="int4")):
         with pytest.raises(ValueError):
             cb.IrrepsNorm("4x0e", **bad)
     with pytest.raises(ValueError, match="gate"):
@@ -57,7 +57,7 @@ def _args(mode, blocks=((4, 1), (4, 3)), rows=3, **kw):
 
 @pytest.mark.parametrize("change,text", [
     (dict(struct_bytes=8), "another argument block"), (dict(mode=4), "mode"), (dict(gate=3), "gate"), (dict(dtype=7), "element type"),
-    (dict(num_blocks=0), "irrep blocks"), (dict(num_blocks=65), "irrep blocks"), (dict(rows=-1), "rows"), (dict(eps=0.0), "eps"),
+    (dict(num_blocks=0), "irrep blocks"), (dict(num_blocks=65), "irrep blocks"), (dict(rows=-1), "rows"), (dict(eps=0.0), "eps"), (dict(eps=float("inf")), "eps"), (dict(eps=1e-39), "eps"), (dict(eps=1e-39, dtype=1), "null weight"),
     (dict(codes=16, dtype=1), "8 bits"), (dict(stats_stride=5), "stride"), (dict(), "null weight"), (dict(weight=16), "operand"),
     (dict(weight=16, x=16, ldx=8), "operand"), (dict(weight=16, x=16, ldx=16), "null result"),
     (dict(weight=16, x=16, ldx=16, norm=16, codes=16, ld_codes=16), "codes need"),
