@@ -138,6 +138,16 @@ def test_residual_norm_in_8_bits(irreps, rows, seed):
     _residual(irreps, rows, F32, cb.mul_ir, "silu", True, "int8", seed)
 
 
+@pytest.mark.parametrize("irreps,rows", [("5x0e+3x1o+2x2e", 70001), ("48x0e+32x1o", 30011), ("64x0e+7x1o", 45003)])
+def test_many_stages_per_warp(irreps, rows):
+    """More rows than all warps of a GPU take at a time, the last stages incomplete; dense rows of even and odd length."""
+    _norm(irreps, rows, F32, cb.mul_ir)
+    _norm(irreps, rows, BF16, cb.ir_mul, "int8")
+    _residual(irreps, rows, F32, cb.ir_mul, "silu", True)
+    _residual(irreps, rows, F16, cb.mul_ir, "sigmoid", False)
+    _residual(irreps, rows, F32, cb.mul_ir, None, False, "int8")
+
+
 @pytest.mark.parametrize("param_dtype", [BF16, F16])
 def test_parameters_of_16_bits(param_dtype):
     _norm("64x0e+32x1o", 300, F32, cb.mul_ir, param_dtype=param_dtype)
