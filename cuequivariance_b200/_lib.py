@@ -390,6 +390,9 @@ def status_word(device):
     bounded waits write a non-zero code there instead of hanging (1: a bulk copy of the channelwise
     staging variant ran out of time, 2: a wait inside a tensor-core kernel did).  Launches never read
     it back (that would synchronise); call :func:`check_status` at a point where a sync is acceptable."""
+    t = _status_words.get(device)
+    if t is not None:
+        return t
     import torch
 
     dev = torch.device(device)

@@ -216,7 +216,7 @@ class _FusedLinear(torch.autograd.Function):
         parts = None
         if which == "gw":
             n = L.cueq_b200_linear_gw_floats(C.byref(a))
-            parts = torch.empty(max(n, 0), dtype=torch.float32, device=x.device)
+            parts = out.new_empty(max(n, 0))
             a.parts, a.parts_floats = parts.data_ptr(), n
         name = ("linear" if len(bounds) == 2 else "indexed_linear") + "_f32x3" + ("_gx" if transposed else "" if which == "map" else f"_{which}")
         with _lib.on_device(x.device), profiling.kernel(name):
@@ -265,8 +265,8 @@ class _FusedLinear8(torch.autograd.Function):
         values = steps = None
         if ctx.needs_input_grad[2]:
             rows, paths = x.shape[0], plan["paths"]
-            values = torch.empty((rows, sum(u * d for (_, u, _, _, _, d, _) in paths)), dtype=torch.int8, device=x.device)
-            steps = torch.empty((len(paths), (rows + 3) // 4 * 4), dtype=torch.float32, device=x.device)
+            values = x.new_empty((rows, sum(u * d for (_, u, _, _, _, d, _) in paths)), dtype=torch.int8)
+            steps = x.new_empty((len(paths), (rows + 3) // 4 * 4))
             _FusedLinear._launch(plan, "pack", bounds, x, x, x, codes=(values, steps))
         ctx.save_for_backward(weight, values, steps)
         return out

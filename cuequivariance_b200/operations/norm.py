@@ -39,6 +39,11 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous()
 
 
+def _features(like: torch.Tensor, width: int) -> torch.Tensor:
+    """Dense rows of ``width`` values for the rows of ``like``."""
+    return torch.empty_like(like) if like.shape[1] == width and like.is_contiguous() else like.new_empty((like.shape[0], width))
+
+
 class _Block:
     """What the modules share: the irreps' blocks, the layout and the launches."""
 
@@ -120,19 +125,18 @@ class _Block:
         a.x, a.ldx = x.data_ptr(), x.stride(0)
         out = norm = codes = stats = None
         if y is not None:
-            out = torch.empty((x.shape[0], self.dim), dtype=x.dtype, device=x.device)
+            out = _features(x, self.dim)
             a.y, a.ldy, a.scale, a.out = y.data_ptr(), y.stride(0), s.data_ptr(), out.data_ptr()
         if g is not None:
             a.g, a.ldg = g.data_ptr(), g.stride(0)
         if w is not None:
-            norm = torch.empty((x.shape[0], self.dim), dtype=x.dtype, device=x.device)
+            norm = _features(x, self.dim)
             a.weight, a.norm = w.data_ptr(), norm.data_ptr()
         if keep:
-            stats = torch.empty((x.shape[0], len(self.blocks), self.stats_stride),
-                                dtype=torch.float64 if x.dtype == torch.float64 else torch.float32, device=x.device)
+            stats = x.new_empty((x.shape[0], len(self.blocks), self.stats_stride), dtype=torch.float64 if x.dtype == torch.float64 else torch.float32)
             a.stats = stats.data_ptr()
             if self.int8:
-                codes = torch.empty((x.shape[0], self.code_bytes), dtype=torch.int8, device=x.device)
+                codes = x.new_empty((x.shape[0], self.code_bytes), dtype=torch.int8)
                 a.codes, a.ld_codes = codes.data_ptr(), self.code_bytes
         if x.shape[0]:
             self.launch("forward", a, x.device)
@@ -145,38 +149,34 @@ class _Block:
         s, w = (None if t is None else t.contiguous() for t in (s, w))
         a = self.arguments(mode, like, s if s is not None else w)
         rows, dx, dy, dg, ds, dw = like.shape[0], go, None, None, None, None
-        held = []
-
-        def operand(t):
-            held.append(_rows(t))
-            return held[-1].data_ptr(), held[-1].stride(0)
-
+        # copies of operands live until the launch
+        go, gn, y, g, h = (None if t is None else _rows(t) for t in (go, gn, y, g, h))
         if go is not None:
-            a.go, a.ldgo = operand(go)
+            a.go, a.ldgo = go.data_ptr(), go.stride(0)
         if mode & _lib.NORM_BRANCH:
-            dy = torch.empty((rows, self.dim), dtype=like.dtype, device=like.device)
+            dy = _features(like, self.dim)
             ds = torch.empty_like(s)
             a.scale, a.dy, a.dscale = s.data_ptr(), dy.data_ptr(), ds.data_ptr()
             if y is not None:
-                a.y, a.ldy = operand(y)
+                a.y, a.ldy = y.data_ptr(), y.stride(0)
             if self.gate:
-                dg = torch.empty((rows, self.channels), dtype=like.dtype, device=like.device)
+                dg = _features(like, self.channels)
                 a.dg = dg.data_ptr()
                 if g is not None:
-                    a.g, a.ldg = operand(g)
+                    a.g, a.ldg = g.data_ptr(), g.stride(0)
         if mode & _lib.NORM_ALONE:
-            a.gn, a.ldgn = operand(gn)
-            dx = torch.empty((rows, self.dim), dtype=like.dtype, device=like.device)
+            a.gn, a.ldgn = gn.data_ptr(), gn.stride(0)
+            dx = _features(like, self.dim)
             dw = torch.empty_like(w)
             a.weight, a.dx, a.dweight = w.data_ptr(), dx.data_ptr(), dw.data_ptr()
             if h is not None:
-                a.h, a.ldh = operand(h)
+                a.h, a.ldh = h.data_ptr(), h.stride(0)
         a.stats = stats.data_ptr()
         if codes is not None:
             a.codes, a.ld_codes = codes.data_ptr(), self.code_bytes
         if rows:
             n = max(_lib.lib().cueq_b200_norm_parts(C.byref(a)), 0)
-            parts = torch.empty(n, dtype=stats.dtype, device=like.device)
+            parts = stats.new_empty(n)
             a.parts, a.parts_values = parts.data_ptr(), n
             self.launch("backward", a, like.device)
         else:
@@ -220,8 +220,10 @@ _gradients_once = torch.autograd.function.once_differentiable(_gradients)
 
 
 def _run(block: _Block, x, y, g, s, w):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, g, s, w)):
-        return _Norm.apply(block, x, y, g, s, w)
+    if torch.is_grad_enabled():
+        for t in (x, y, g, s, w):
+            if t is not None and t.requires_grad:
+                return _Norm.apply(block, x, y, g, s, w)
     out, norm, _, _ = block.forward(False, x, y, g, s, w)
     return tuple(t for t in (out, norm) if t is not None)
 
