@@ -236,10 +236,10 @@ __global__ void __launch_bounds__(kSumChannels * kSumRows) sum_kernel(const __gr
 
 Kernel pick_kernel(int dtype, int mode, bool q8, bool mul_ir, bool backward) {
   switch (dtype) {
-    case CUEQ_F32: return pick_f32(mode, q8, mul_ir, backward);
-    case CUEQ_F64: return pick_f64(mode, q8, mul_ir, backward);
-    case CUEQ_BF16: return pick_bf16(mode, q8, mul_ir, backward);
-    default: return pick_f16(mode, q8, mul_ir, backward);
+    case CUEQ_F32: return q8 ? pick_f32_codes(mode, mul_ir, backward) : pick_f32(mode, mul_ir, backward);
+    case CUEQ_F64: return pick_f64(mode, mul_ir, backward);
+    case CUEQ_BF16: return q8 ? pick_bf16_codes(mode, mul_ir, backward) : pick_bf16(mode, mul_ir, backward);
+    default: return q8 ? pick_f16_codes(mode, mul_ir, backward) : pick_f16(mode, mul_ir, backward);
   }
 }
 

@@ -1,4 +1,4 @@
-// The norm kernels of one element type (norm_kernels.cuh); a file each, so that they compile side by side.
+// The norm kernels of one element type (norm_kernels.cuh).
 #include "norm_kernels.cuh"
 
-cueq_norm::Kernel cueq_norm::pick_bf16(int mode, bool q8, bool mul_ir, bool backward) { return pick<__nv_bfloat16, float>(mode, q8, mul_ir, backward); }
+cueq_norm::Kernel cueq_norm::pick_bf16(int mode, bool mul_ir, bool backward) { return pick<__nv_bfloat16, float, false>(mode, mul_ir, backward); }

@@ -1,4 +1,4 @@
-// The norm kernels of one element type (norm_kernels.cuh); a file each, so that they compile side by side.
+// The norm kernels of one element type (norm_kernels.cuh).
 #include "norm_kernels.cuh"
 
-cueq_norm::Kernel cueq_norm::pick_f16(int mode, bool q8, bool mul_ir, bool backward) { return pick<__half, float>(mode, q8, mul_ir, backward); }
+cueq_norm::Kernel cueq_norm::pick_f16(int mode, bool mul_ir, bool backward) { return pick<__half, float, false>(mode, mul_ir, backward); }

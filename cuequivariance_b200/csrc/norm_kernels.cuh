@@ -405,9 +405,12 @@ __device__ __forceinline__ void warp_sums(M (&s)[R], int lane, int lanes) {
 }
 template <bool NARROW>
 __device__ __forceinline__ unsigned warp_top(unsigned v, int lanes) {
-  if (!NARROW) return __reduce_max_sync(0xffffffffu, v);
-  for (int o = lanes >> 1; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+  if constexpr (NARROW) {
+    for (int o = lanes >> 1; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  } else {
+    return __reduce_max_sync(0xffffffffu, v);
+  }
 }
 
 template <class T, class M, int DIM, bool MUL_IR, int K, int R, bool NARROW>
@@ -1092,16 +1095,15 @@ Kernel pick(int mode, bool backward) {
     return mode == kBranch ? backward_kernel<T, M, kBranch, Q8, MUL_IR> : mode == kNorm ? backward_kernel<T, M, kNorm, Q8, MUL_IR> : backward_kernel<T, M, kBoth, Q8, MUL_IR>;
   return mode == kBranch ? forward_kernel<T, M, kBranch, Q8, MUL_IR> : mode == kNorm ? forward_kernel<T, M, kNorm, Q8, MUL_IR> : forward_kernel<T, M, kBoth, Q8, MUL_IR>;
 }
-template <class T, class M>
-Kernel pick(int mode, bool q8, bool mul_ir, bool backward) {
-  if constexpr (sizeof(M) == 4) {
-    if (q8) return mul_ir ? pick<T, M, true, true>(mode, backward) : pick<T, M, true, false>(mode, backward);
-  }
-  return mul_ir ? pick<T, M, false, true>(mode, backward) : pick<T, M, false, false>(mode, backward);
-}
-Kernel pick_f32(int mode, bool q8, bool mul_ir, bool backward);
-Kernel pick_f64(int mode, bool q8, bool mul_ir, bool backward);
-Kernel pick_bf16(int mode, bool q8, bool mul_ir, bool backward);
-Kernel pick_f16(int mode, bool q8, bool mul_ir, bool backward);
+template <class T, class M, bool Q8>
+Kernel pick(int mode, bool mul_ir, bool backward) { return mul_ir ? pick<T, M, Q8, true>(mode, backward) : pick<T, M, Q8, false>(mode, backward); }
+// a file each, so that they compile side by side; _codes: activations in 8 bits
+Kernel pick_f32(int mode, bool mul_ir, bool backward);
+Kernel pick_f32_codes(int mode, bool mul_ir, bool backward);
+Kernel pick_f64(int mode, bool mul_ir, bool backward);
+Kernel pick_bf16(int mode, bool mul_ir, bool backward);
+Kernel pick_bf16_codes(int mode, bool mul_ir, bool backward);
+Kernel pick_f16(int mode, bool mul_ir, bool backward);
+Kernel pick_f16_codes(int mode, bool mul_ir, bool backward);
 
 }  // namespace cueq_norm

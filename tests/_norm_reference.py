@@ -88,12 +88,14 @@ def reference(blocks, mul_ir, eps, gate, int8, x, y=None, g=None, s=None, w=None
         cmag = cot.abs()
         if gn is not None:
             hk = kept(h, int8)
+            # h = x + branch is off by as much as its terms are, however small it is itself, and r(h) by the mean of that along h
+            hm = (hk.abs() if y is None else hmag) * (1 + (rh**2 * (hmag * h.abs()).flatten(1).mean(1)[:, None, None] if y is not None else 0))
             p = (gnb * hk).sum(2, keepdim=True)
-            pm = (gnb * hk).abs().sum(2, keepdim=True)
+            pm = (gnb.abs() * hm).sum(2, keepdim=True)
             put("dw", (rh * p).sum((0, 2)), (rh * pm).sum((0, 2)), "channels")
             mean, mm = (wc * p).sum(1, keepdim=True) / n, (wc.abs() * pm).sum(1, keepdim=True) / n
             cot = cot + rh * (wc * gnb - hk * rh**2 * mean)
-            cmag = cmag + rh * ((wc * gnb).abs() + hk.abs() * rh**2 * mm)
+            cmag = cmag + rh * ((wc * gnb).abs() + hm * rh**2 * mm)
             put("dx", cot, cmag, "rows")
         elif y is not None:
             put("dx", cot, cmag, "rows")
