@@ -178,8 +178,7 @@ class _FusedLinear(torch.autograd.Function):
 
     @staticmethod
     def _launch(plan, which, bounds, x, w, out, transposed=0, codes=None):
-        """``which``: map, gw (``w``: cotangent rows), pack (``w``, ``out``: anything).  ``codes``: written by pack; gw reads them in place
-        of ``x``."""
+        """``which``: map or gw (``w``: cotangent rows).  ``codes``: of x, written behind a map; gw reads them in place of ``x``."""
         import ctypes as C
 
         if x.shape[0] == 0:
@@ -210,25 +209,31 @@ class _FusedLinear(torch.autograd.Function):
             c = _lib.LinearCodes()
             c.struct_bytes, c.rows = C.sizeof(c), values.shape[0]
             c.codes, c.ld_codes, c.steps, c.ld_steps = values.data_ptr(), values.shape[1], steps.data_ptr(), steps.shape[1]
-            fn = L.cueq_b200_linear_pack if which == "pack" else L.cueq_b200_linear_gw_codes
-        else:
-            fn = L.cueq_b200_linear_map if which == "map" else L.cueq_b200_linear_gw
         parts = None
         if which == "gw":
             n = L.cueq_b200_linear_gw_floats(C.byref(a))
             parts = out.new_empty(max(n, 0))
             a.parts, a.parts_floats = parts.data_ptr(), n
-        name = ("linear" if len(bounds) == 2 else "indexed_linear") + "_f32x3" + ("_gx" if transposed else "" if which == "map" else f"_{which}")
-        with _lib.on_device(x.device), profiling.kernel(name):
+        name = ("linear" if len(bounds) == 2 else "indexed_linear") + "_f32x3" + ("_gx" if transposed else "" if which == "map" else "_gw")
+        with _lib.on_device(x.device):
             stream = torch._C._cuda_getCurrentRawStream(x.device.index)
-            _lib.check(fn(C.byref(a), stream) if c is None else fn(C.byref(a), C.byref(c), stream))
+            with profiling.kernel(name):
+                if which == "map":
+                    _lib.check(L.cueq_b200_linear_map(C.byref(a), stream))
+                elif c is None:
+                    _lib.check(L.cueq_b200_linear_gw(C.byref(a), stream))
+                else:
+                    _lib.check(L.cueq_b200_linear_gw_codes(C.byref(a), C.byref(c), stream))
+            if which == "map" and c is not None:
+                with profiling.kernel(name + "_pack"):
+                    _lib.check(L.cueq_b200_linear_pack(C.byref(a), C.byref(c), stream))
 
     @staticmethod
-    def _apply(plan, bounds, weight, x):
+    def _apply(plan, bounds, weight, x, codes=None):
         x, weight = _aligned(x), _aligned(weight)
         all_rows = bounds[0] == 0 and bounds[-1] == x.shape[0]
         out = (torch.empty if plan["full_out"] and all_rows else torch.zeros)((x.shape[0], plan["out_size"]), dtype=torch.float32, device=x.device)
-        _FusedLinear._launch(plan, "map", bounds, x, weight, out)
+        _FusedLinear._launch(plan, "map", bounds, x, weight, out, codes=codes)
         return out, weight, x, all_rows
 
     @staticmethod
@@ -260,14 +265,11 @@ class _FusedLinear8(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, plan, bounds, weight, x):
-        out, weight, x, ctx.all_rows = _FusedLinear._apply(plan, bounds, weight, x)
-        ctx.plan, ctx.bounds, ctx.rows = plan, bounds, x.shape[0]
-        values = steps = None
-        if ctx.needs_input_grad[2]:
-            rows, paths = x.shape[0], plan["paths"]
-            values = x.new_empty((rows, sum(u * d for (_, u, _, _, _, d, _) in paths)), dtype=torch.int8)
-            steps = x.new_empty((len(paths), (rows + 3) // 4 * 4))
-            _FusedLinear._launch(plan, "pack", bounds, x, x, x, codes=(values, steps))
+        rows, paths = x.shape[0], plan["paths"]
+        values = x.new_empty((rows, sum(u * d for (_, u, _, _, _, d, _) in paths)), dtype=torch.int8)
+        steps = x.new_empty((len(paths), (rows + 3) // 4 * 4))
+        out, weight, _, ctx.all_rows = _FusedLinear._apply(plan, bounds, weight, x, (values, steps))
+        ctx.plan, ctx.bounds, ctx.rows = plan, bounds, rows
         ctx.save_for_backward(weight, values, steps)
         return out
 
