@@ -25,7 +25,9 @@
 // 64x(0e+1o) in bfloat16 115 + 149 us (floor 72 + 82), 0.7 of the issue slots used; the gate's exponential and the sums over the warp
 // are most of them.
 //
-// Sums, statistics and all arithmetic are in 32 bits for 16- and 32-bit data, in 64 for 64-bit data; results are rounded once.
+// Sums, statistics and all arithmetic are in 32 bits for 16- and 32-bit data, in 64 for 64-bit data; results are rounded once.  h is
+// rounded on its way out, like every result, and the backward pass of the norm behind a branch reads it so: half a step of 16 bits off, as
+// the gradient that it enters is itself.
 //
 // Kept in 8 bits (Q8): codes per (row, irrep block), see code_step in common.cuh.  r stays that of the exact values; the gradients of a block
 // that holds an infinity or NaN are NaN.

@@ -243,7 +243,7 @@ class IrrepsNorm(torch.nn.Module):
     (ones at first).  float64 features go with float64 weights; others with weights of any other type.  Arithmetic, statistics and
     sums are in 32 bits (64 for float64); results are rounded once.  Rows may lie further apart than their width.
 
-    ``saved_activations="int8"`` keeps x in 8 bits for the backward pass, per row and irrep block with a step of a power of two (off by at most
+    ``saved_activations="int8"`` (not for float64) keeps x in 8 bits for the backward pass, per row and irrep block with a step of a power of two (off by at most
     1/127 of the block's largest magnitude); the forward result does not change.  First derivatives only."""
 
     def __init__(self, irreps, *, layout=None, eps: float = 1e-5, internal_weights: bool = True, saved_activations: str = "full",
