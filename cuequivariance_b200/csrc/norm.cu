@@ -15,6 +15,8 @@ constexpr int kStageBytes = 4096;        // rows are put together up to about th
 
 int element_size(int dtype) { return dtype == CUEQ_F64 ? 8 : dtype == CUEQ_F32 ? 4 : 2; }
 bool gated(const cueq_norm_args* a) { return a->gate != CUEQ_NORM_GATE_NONE && (a->mode & kBranch); }
+// the backward pass forms h again from x (kAgain)
+bool again(const cueq_norm_args* a) { return a->mode == kBoth && !a->codes && element_size(a->dtype) == 2; }
 // a branch whose norm has no cotangent is differentiated alone, with the statistics that both have left
 int stats_per_item(const cueq_norm_args* a) { return a->stats_stride ? a->stats_stride : a->codes && a->mode == kBoth ? 8 : 4; }
 
@@ -56,7 +58,7 @@ void set_routes(const cueq_norm_args* a, bool backward, Params* p, bool whole, b
     return even && ld * size % 16 == 0 ? kRows : kPlain;
   };
   const int64_t d = p->dim_total, c = p->channels;
-  p->route[tX] = route(a->x, a->ldx, d); p->route[tY] = route(a->y, a->ldy, d); p->route[tH] = route(a->h, a->ldh, d);
+  p->route[tX] = route(a->x, a->ldx, d); p->route[tY] = route(a->y, a->ldy, d); p->route[tH] = again(a) ? p->route[tX] : route(a->h, a->ldh, d);
   p->route[tGo] = route(a->go, a->ldgo, d); p->route[tGn] = route(a->gn, a->ldgn, d); p->route[tG] = route(a->g, a->ldg, c);
   p->route[tOut] = route(a->out, d, d); p->route[tNorm] = route(a->norm, d, d);
   p->route[tDx] = route(a->dx, d, d); p->route[tDy] = route(a->dy, d, d); p->route[tDg] = route(a->dg, c, c);
@@ -261,7 +263,7 @@ int launch(const cueq_norm_args* a, bool backward, void* stream) {
     if (!operand(a->x, a->ldx, width) || (branch && !operand(a->y, a->ldy, width))) return cueq::fail("norm: an operand is missing or its rows overlap");
     if ((branch && !a->out) || (norm && !a->norm)) return cueq::fail("norm: null result");
   } else {
-    if (!q8 && ((branch && !operand(a->y, a->ldy, width)) || (norm && !operand(a->h, a->ldh, width)))) return cueq::fail("norm: a kept operand is missing or its rows overlap");
+    if (!q8 && ((branch && !operand(a->y, a->ldy, width)) || (norm && !(again(a) ? operand(a->x, a->ldx, width) : operand(a->h, a->ldh, width))))) return cueq::fail("norm: a kept operand is missing or its rows overlap");
     if (norm ? !operand(a->gn, a->ldgn, width) : !operand(a->go, a->ldgo, width)) return cueq::fail("norm: a cotangent is missing or its rows overlap");
     if (a->mode == kBoth && a->go && !operand(a->go, a->ldgo, width)) return cueq::fail("norm: a cotangent's rows overlap");
     if ((branch && !a->dy) || (norm && !a->dx) || (gated(a) && !a->dg)) return cueq::fail("norm: null result");
@@ -270,6 +272,7 @@ int launch(const cueq_norm_args* a, bool backward, void* stream) {
   }
   p.x = a->x; p.y = a->y; p.g = a->g; p.h = a->h; p.go = a->go; p.gn = a->gn;
   p.ldx = a->ldx; p.ldy = a->ldy; p.ldg = a->ldg; p.ldh = a->ldh; p.ldgo = a->ldgo; p.ldgn = a->ldgn;
+  if (again(a)) { p.h = a->x; p.ldh = a->ldx; }
   p.s = a->scale; p.w = a->weight;
   p.out = a->out; p.norm = a->norm; p.dx = a->dx; p.dy = a->dy; p.dg = a->dg;
   p.codes = (signed char*)a->codes; p.ldc = a->ld_codes;

@@ -25,9 +25,10 @@
 // 64x(0e+1o) in bfloat16 115 + 149 us (floor 72 + 82), 0.7 of the issue slots used; the gate's exponential and the sums over the warp
 // are most of them.
 //
-// Sums, statistics and all arithmetic are in 32 bits for 16- and 32-bit data, in 64 for 64-bit data; results are rounded once.  h is
-// rounded on its way out, like every result, and the backward pass of the norm behind a branch reads it so: half a step of 16 bits off, as
-// the gradient that it enters is itself.
+// Sums, statistics and all arithmetic are in 32 bits for 16- and 32-bit data, in 64 for 64-bit data; results are rounded once.  In 16 bits
+// h is rounded on its way out, so the backward pass of the norm behind a branch reads x in its place and forms h again (kAgain): as many bytes,
+// and the gradients of s and w, which may have 32 bits, are not half a step of 16 bits off.  Backward in bfloat16 with h read as rounded and now:
+// 32,768 rows of 128x(0e+1o+2e+3o) 208 and 217 us, 262,144 of 64x(0e+1o) 350 and 338, 32,768 of 256x(0e+1o), in loops, 246 and 279.
 //
 // Kept in 8 bits (Q8): codes per (row, irrep block), see code_step in common.cuh.  r stays that of the exact values; the gradients of a block
 // that holds an infinity or NaN are NaN.
@@ -131,7 +132,7 @@ __host__ __device__ inline Stage forward_stage(const Params& p, const Slice& s, 
   t.total = at;
   return t;
 }
-// backward: a = go (then dx behind a branch with a norm, dy behind one without), b = gn (then dy, or dx for the norm alone), c = h,
+// backward: a = go (then dx behind a branch with a norm, dy behind one without), b = gn (then dy, or dx for the norm alone), c = h (kAgain: x),
 // d = y, g = gates, dg = their gradient (over g where that is not in codes), st = statistics
 __host__ __device__ inline Stage backward_stage(const Params& p, const Slice& s, int mode, bool q8, int size, int stat_bytes) {
   Stage t{};
@@ -300,6 +301,9 @@ __device__ __forceinline__ void forward_item(const View<M>& c, T* __restrict__ x
   }
 }
 
+// h of the norm behind a branch is formed again from x (in its place), y and the gates
+template <class T, class M, int MODE, bool Q8> constexpr bool kAgain = MODE == kBoth && !Q8 && sizeof(T) < sizeof(M);
+
 // K: type of what was kept (T or codes).  r (r c) stays in range: r^2 <= 1 / eps, and r >= 1e-19 while the sum of squares is finite.
 template <class T, class M, class K, int MODE, bool Q8, int DIM, bool MUL_IR>
 __device__ __forceinline__ void backward_item(const View<M>& c, T* __restrict__ go, T* __restrict__ gn, const K* __restrict__ h, const K* __restrict__ y, const K* g, T* dg,
@@ -307,14 +311,21 @@ __device__ __forceinline__ void backward_item(const View<M>& c, T* __restrict__ 
   const M *__restrict__ cs = c.s, *__restrict__ cw = c.w;
   M *__restrict__ cc = c.a, *__restrict__ acc_s = c.acc_s, *__restrict__ acc_w = c.acc_w;
   M rh = M(0), qh = M(0);
+  // channel u, element `at` of what was normalised
+  auto normed = [&](int u, int at) { return kAgain<T, M, MODE, Q8> ? to<M>(h[at]) + cc[u] * to<M>(y[at]) : to<M>(h[at]); };
   if (MODE & kNorm) {
     rh = stats[MODE == kBoth ? 1 : 0];
     const M step = Q8 ? stats[MODE == kBoth ? 4 : 2] : M(1);
     const M rs = rh * step;
     M dot = M(0);
     CUEQ_CHANNELS {
+      if (kAgain<T, M, MODE, Q8>) {
+        M v = M(1), dv;
+        if (c.gated) activation<T>(c.gate, to<M>(g[u]), v, dv);
+        cc[u] = cs[u] * v * stats[0];
+      }
       M p = M(0);
-      CUEQ_COMPONENTS p += to<M>(gn[CUEQ_AT]) * to<M>(h[CUEQ_AT]);
+      CUEQ_COMPONENTS p += to<M>(gn[CUEQ_AT]) * normed(u, CUEQ_AT);
       p *= rs;
       acc_w[u] += p;
       dot += cw[u] * p;
@@ -338,7 +349,7 @@ __device__ __forceinline__ void backward_item(const View<M>& c, T* __restrict__ 
     const M b = MODE == kBoth ? cw[u] * rh : M(0), s = cs[u];
     CUEQ_COMPONENTS {
       M o = MODE == kBranch || has_go ? to<M>(go[CUEQ_AT]) : M(0);
-      if (MODE == kBoth) o += b * to<M>(gn[CUEQ_AT]) - qh * to<M>(h[CUEQ_AT]);
+      if (MODE == kBoth) o += b * to<M>(gn[CUEQ_AT]) - qh * normed(u, CUEQ_AT);
       if (kPut) go[CUEQ_AT] = from<T>(o);
       p += o * to<M>(y[CUEQ_AT]);
     }
@@ -354,7 +365,7 @@ __device__ __forceinline__ void backward_item(const View<M>& c, T* __restrict__ 
     const M a = cc[u], b = MODE == kBoth ? cw[u] * rh : M(0);
     CUEQ_COMPONENTS {
       M o = kPut || MODE == kBranch || has_go ? to<M>(go[CUEQ_AT]) : M(0);
-      if (MODE == kBoth && !kPut) o += b * to<M>(gn[CUEQ_AT]) - qh * to<M>(h[CUEQ_AT]);
+      if (MODE == kBoth && !kPut) o += b * to<M>(gn[CUEQ_AT]) - qh * normed(u, CUEQ_AT);
       const T dy = from<T>(a * o - q * to<M>(y[CUEQ_AT]));
       if (MODE == kBoth && !kPut) go[CUEQ_AT] = from<T>(o);
       (MODE == kBoth ? gn : go)[CUEQ_AT] = dy;
@@ -443,6 +454,20 @@ struct Short {
           if (MUL_IR) v[q][(j * K + k) / DIM][(j * K + k) % DIM] = to<M>(x.v[k]);
           else v[q][k][j] = to<M>(x.v[k]);
         }
+      }
+    }
+  }
+  // v += a times a row of values, one factor per channel
+  template <class E>
+  __device__ __forceinline__ void add_scaled(const E* row, const M (&a)[K], M (&v)[K][DIM]) const {
+    const Vec<E, K>* e = reinterpret_cast<const Vec<E, K>*>(row);
+#pragma unroll
+    for (int j = 0; j < DIM; ++j) {
+      const Vec<E, K> x = e[at(j)];
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (MUL_IR) v[(j * K + k) / DIM][(j * K + k) % DIM] += a[(j * K + k) / DIM] * to<M>(x.v[k]);
+        else v[k][j] += a[k] * to<M>(x.v[k]);
       }
     }
   }
@@ -593,11 +618,30 @@ template <class T, class M, class K8, int MODE, bool Q8, int DIM, bool MUL_IR, i
 __device__ __forceinline__ void backward_short(const View<M>& c, int left, Rows<T> go, Rows<T> gn, Rows<K8> h, Rows<K8> y, Rows<K8> g, Rows<T> dg,
                                                Rows<M> stats, bool has_go) {
   const Short<T, M, DIM, MUL_IR, K, R, NARROW> w(c, left);
-  M o[R][K][DIM], v[R][K][DIM], dot[R], sum[K];
+  constexpr bool again = kAgain<T, M, MODE, Q8>;
+  M o[R][K][DIM], v[R][K][DIM], dot[R], sum[K], s[K];
+  M act[R][K], dact[R][K];                               // again: kept from one use to the other (computed twice: 311 us for 217 with 128x(0e+1o+2e+3o))
   if (MODE & kNorm) {
     M rh[R], step[R], b[K];
     w.load(gn, o);
     w.load(h, v);
+    if constexpr (again) {                               // v is x
+      w.channels(c.s, s);
+#pragma unroll
+      for (int q = 0; q < R; ++q) {
+        const M r1 = stats[w.row(q)][0];
+        M gate[K], ar[K];
+        if (c.gated) w.channels(g[w.row(q)], gate);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          M e = M(1), de = M(0);
+          if (c.gated) activation<T>(c.gate, gate[k], e, de);
+          act[q][k] = e; dact[q][k] = de;
+          ar[k] = s[k] * e * r1;
+        }
+        w.add_scaled(y[w.row(q)], ar, v[q]);
+      }
+    }
     w.channels(c.w, b);
 #pragma unroll
     for (int k = 0; k < K; ++k) sum[k] = M(0);
@@ -645,9 +689,9 @@ __device__ __forceinline__ void backward_short(const View<M>& c, int left, Rows<
   } else {
     w.load(go, o);
   }
-  M r[R], step[R], a[R][K], s[K];
+  M r[R], step[R], a[R][K];
   w.load(y, v);
-  w.channels(c.s, s);
+  if (!again) w.channels(c.s, s);
 #pragma unroll
   for (int k = 0; k < K; ++k) sum[k] = M(0);
 #pragma unroll
@@ -657,12 +701,13 @@ __device__ __forceinline__ void backward_short(const View<M>& c, int left, Rows<
     step[q] = Q8 ? st[2] : M(1);
     dot[q] = M(0);
     M gate[K], de[K];
-    if (c.gated) w.channels(g[w.row(q)], gate);
+    if (c.gated && !again) w.channels(g[w.row(q)], gate);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       M e = M(1), p = M(0);
       de[k] = M(0);
-      if (c.gated) activation<T>(c.gate, Q8 ? gate[k] * st[3] : gate[k], e, de[k]);
+      if constexpr (again) { e = act[q][k]; de[k] = dact[q][k]; }
+      else if (c.gated) activation<T>(c.gate, Q8 ? gate[k] * st[3] : gate[k], e, de[k]);
 #pragma unroll
       for (int i = 0; i < DIM; ++i) p += o[q][k][i] * v[q][k][i];
       p *= r[q] * step[q];

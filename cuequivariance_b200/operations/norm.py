@@ -23,6 +23,7 @@ from ..irreps import Irreps, IrrepsLayout
 _NAMES = {_lib.NORM_BRANCH: "gated_residual_", _lib.NORM_ALONE: "irreps_norm_", _lib.NORM_BOTH: "gated_residual_norm_"}
 SAVED_ACTIVATIONS = ("full", "int8")
 _TYPES = (torch.float32, torch.float64, torch.bfloat16, torch.float16)
+_ROUNDED = (torch.bfloat16, torch.float16)
 
 
 def check_saved_activations(value: str) -> bool:
@@ -142,8 +143,17 @@ class _Block:
             self.launch("forward", a, x.device)
         return out, norm, codes, stats
 
+    def kept(self, x, y, g, out, codes):
+        """(y, g, h) for the backward pass, None where they are in codes or not read.  ``h``: what was normalised; behind a branch in 16
+        bits, where the result has been rounded, x, from which the kernel forms it again."""
+        if codes is not None:
+            return None, None, None
+        if self.mode == _lib.NORM_BOTH:
+            return y, g, x if x.dtype in _ROUNDED else out
+        return y, g, x if self.mode == _lib.NORM_ALONE else None
+
     def backward(self, go, gn, y, g, h, codes, stats, s, w):
-        """(dx, dy, dg, ds, dw); ``y``, ``g``, ``h`` are None where they were kept in codes."""
+        """(dx, dy, dg, ds, dw); ``y``, ``g``, ``h`` as ``kept`` returned them."""
         mode = self.mode if gn is not None else _lib.NORM_BRANCH      # a norm without a cotangent does not count
         like = gn if gn is not None else go
         s, w = (None if t is None else t.contiguous() for t in (s, w))
@@ -170,7 +180,7 @@ class _Block:
             dw = torch.empty_like(w)
             a.weight, a.dx, a.dweight = w.data_ptr(), dx.data_ptr(), dw.data_ptr()
             if h is not None:
-                a.h, a.ldh = h.data_ptr(), h.stride(0)
+                a.h, a.ldh = a.x, a.ldx = h.data_ptr(), h.stride(0)
         a.stats = stats.data_ptr()
         if codes is not None:
             a.codes, a.ld_codes = codes.data_ptr(), self.code_bytes
@@ -185,18 +195,15 @@ class _Block:
 
 
 class _Norm(torch.autograd.Function):
-    """One pass over the rows each way.  Kept for the backward pass: the statistics and y, g, h (alone: x) as they are, or their
-    codes."""
+    """One pass over the rows each way.  Kept for the backward pass: the statistics and y, g, h (alone, or behind a branch in 16 bits:
+    x) as they are, or their codes."""
 
     @staticmethod
     def forward(ctx, block, x, y, g, s, w):
         out, norm, codes, stats = block.forward(True, x, y, g, s, w)
         ctx.block = block
         ctx.set_materialize_grads(False)
-        if codes is not None:
-            ctx.save_for_backward(None, None, None, codes, stats, s, w)
-        else:
-            ctx.save_for_backward(y, g, {_lib.NORM_BRANCH: None, _lib.NORM_ALONE: x, _lib.NORM_BOTH: out}[block.mode], None, stats, s, w)
+        ctx.save_for_backward(*block.kept(x, y, g, out, codes), codes, stats, s, w)
         return tuple(t for t in (out, norm) if t is not None)
 
     @staticmethod
