@@ -15,6 +15,7 @@ import ctypes as C
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib, profiling
 from ..executor import dtype_code
@@ -231,6 +232,8 @@ def _run(block: _Block, x, y, g, s, w):
         for t in (x, y, g, s, w):
             if t is not None and t.requires_grad:
                 return _Norm.apply(block, x, y, g, s, w)
+    if forward_ad._current_level >= 0:
+        return _Norm.apply(block, x, y, g, s, w)          # raises if an operand has a tangent, which needs no requires_grad
     out, norm, _, _ = block.forward(False, x, y, g, s, w)
     return tuple(t for t in (out, norm) if t is not None)
 
@@ -251,7 +254,7 @@ class IrrepsNorm(torch.nn.Module):
     sums are in 32 bits (64 for float64); results are rounded once.  Rows may lie further apart than their width.
 
     ``saved_activations="int8"`` (not for float64) keeps x in 8 bits for the backward pass, per row and irrep block with a step of a power of two (off by at most
-    1/127 of the block's largest magnitude); the forward result does not change.  First derivatives only."""
+    1/127 of the block's largest magnitude); the forward result does not change.  First derivatives only, and none in forward mode."""
 
     def __init__(self, irreps, *, layout=None, eps: float = 1e-5, internal_weights: bool = True, saved_activations: str = "full",
                  device: Optional[torch.device] = None, dtype: Optional[torch.dtype] = None):
