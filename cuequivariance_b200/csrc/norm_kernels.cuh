@@ -818,7 +818,10 @@ __device__ __forceinline__ bool run_stages(const Params& p, int rps, int64_t fir
     __syncwarp();
     if (bytes) bulk_in(stage + jin.at, jin.mem, bytes, full + s);
     jin.mem += jin.step;
-    if (jin.rest || n < rps) copy_rest<true>(in, nin, stage, z, n);
+    if (jin.rest || n < rps) {
+      copy_rest<true>(in, nin, stage, z, n);
+      __syncwarp();                                      // other lanes read what this one has stored; neither a vote nor the barrier orders that
+    }
   };
   const bool two = p.stages == 2;
   if (first < last) load(first, 0);
