@@ -239,8 +239,8 @@ class _FusedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, plan, bounds, weight, x):
         out, weight, x, ctx.all_rows = _FusedLinear._apply(plan, bounds, weight, x)
-        ctx.plan, ctx.bounds = plan, bounds
-        ctx.save_for_backward(weight, x)
+        ctx.plan, ctx.bounds, ctx.rows = plan, bounds, x.shape[0]
+        ctx.save_for_backward(weight, x if ctx.needs_input_grad[2] else None)      # only the weight gradient reads x
         return out
 
     @staticmethod
@@ -251,7 +251,7 @@ class _FusedLinear(torch.autograd.Function):
         gout = _aligned(gout)
         gw = gx = None
         if ctx.needs_input_grad[3]:
-            gx = (torch.empty_like if plan["full_in"] and ctx.all_rows else torch.zeros_like)(x)
+            gx = (torch.empty if plan["full_in"] and ctx.all_rows else torch.zeros)((ctx.rows, plan["in_size"]), dtype=torch.float32, device=gout.device)
             _FusedLinear._launch(plan, "map", bounds, gout, weight, gx, transposed=1)
         if ctx.needs_input_grad[2]:
             # the weights are the blocks of the paths, all of them written; without any row nothing is
