@@ -268,7 +268,8 @@ int launch(const cueq_norm_args* a, bool backward, void* stream) {
     if (a->mode == kBoth && a->go && !operand(a->go, a->ldgo, width)) return cueq::fail("norm: a cotangent's rows overlap");
     if ((branch && !a->dy) || (norm && !a->dx) || (gated(a) && !a->dg)) return cueq::fail("norm: null result");
     const int64_t need = 2 * (int64_t)grid * p.channels;
-    if (a->rows && (!a->parts || a->parts_values < need)) return cueq::fail("norm: the parameters' gradients need room for %lld partial sums", (long long)need);
+    if (a->parts_values < 0 && (a->dscale || a->dweight)) return cueq::fail("norm: the parameters' gradients need partial sums");
+    if (a->rows && a->parts_values >= 0 && (!a->parts || a->parts_values < need)) return cueq::fail("norm: the parameters' gradients need room for %lld partial sums", (long long)need);
   }
   p.x = a->x; p.y = a->y; p.g = a->g; p.h = a->h; p.go = a->go; p.gn = a->gn;
   p.ldx = a->ldx; p.ldy = a->ldy; p.ldg = a->ldg; p.ldh = a->ldh; p.ldgo = a->ldgo; p.ldgn = a->ldgn;
@@ -276,7 +277,7 @@ int launch(const cueq_norm_args* a, bool backward, void* stream) {
   p.s = a->scale; p.w = a->weight;
   p.out = a->out; p.norm = a->norm; p.dx = a->dx; p.dy = a->dy; p.dg = a->dg;
   p.codes = (signed char*)a->codes; p.ldc = a->ld_codes;
-  p.stats = a->stats; p.parts = a->parts;
+  p.stats = a->stats; p.parts = a->parts_values < 0 ? nullptr : a->parts;
   p.rows = a->rows; p.eps = a->eps; p.status = (int*)a->status;
   p.pdtype = a->param_dtype; p.mul_ir = a->mul_ir;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

@@ -78,7 +78,7 @@ struct Params {
   signed char* codes;
   int64_t ldc;
   void* stats;
-  void* parts;
+  void* parts;                       // null: no gradients of the parameters
   int64_t rows;
   double eps;
   int* status;
@@ -1080,6 +1080,7 @@ __device__ __forceinline__ bool backward_slice(const Params& p, const Slice& sl,
     }
   });
   // this warp's sums of the parameters' gradients
+  if (!p.parts) return done;
   M* dst = reinterpret_cast<M*>(p.parts) + (int64_t)blockIdx.x * p.channels + b0.ch;
   const Head head = head_of(sl, MODE, true);
   for (int k = sl.first; k < sl.first + sl.count; ++k) {
@@ -1126,6 +1127,7 @@ __global__ void __launch_bounds__(32, warps_per_sm(sizeof(M))) backward_kernel(c
     int64_t first, last;
     share.rows(p, s, first, last);
     if (first >= last) {                                 // fewer rows than warps: its sums are nothing
+      if (!p.parts) continue;
       const Slice& sl = p.slice[s];
       M* dst = reinterpret_cast<M*>(p.parts) + (int64_t)blockIdx.x * p.channels + p.blk[sl.first].ch;
       for (int u = threadIdx.x; u < sl.channels; u += 32) {

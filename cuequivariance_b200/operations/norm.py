@@ -153,8 +153,8 @@ class _Block:
             return y, g, x if x.dtype in _ROUNDED else out
         return y, g, x if self.mode == _lib.NORM_ALONE else None
 
-    def backward(self, go, gn, y, g, h, codes, stats, s, w):
-        """(dx, dy, dg, ds, dw); ``y``, ``g``, ``h`` as ``kept`` returned them."""
+    def backward(self, go, gn, y, g, h, codes, stats, s, w, need_s, need_w):
+        """(dx, dy, dg, ds, dw); ``y``, ``g``, ``h`` as ``kept`` returned them; ds, dw None where they are not needed."""
         mode = self.mode if gn is not None else _lib.NORM_BRANCH      # a norm without a cotangent does not count
         like = gn if gn is not None else go
         s, w = (None if t is None else t.contiguous() for t in (s, w))
@@ -166,8 +166,10 @@ class _Block:
             a.go, a.ldgo = go.data_ptr(), go.stride(0)
         if mode & _lib.NORM_BRANCH:
             dy = _features(like, self.dim)
-            ds = torch.empty_like(s)
-            a.scale, a.dy, a.dscale = s.data_ptr(), dy.data_ptr(), ds.data_ptr()
+            a.scale, a.dy = s.data_ptr(), dy.data_ptr()
+            if need_s:
+                ds = torch.empty_like(s)
+                a.dscale = ds.data_ptr()
             if y is not None:
                 a.y, a.ldy = y.data_ptr(), y.stride(0)
             if self.gate:
@@ -178,17 +180,21 @@ class _Block:
         if mode & _lib.NORM_ALONE:
             a.gn, a.ldgn = gn.data_ptr(), gn.stride(0)
             dx = _features(like, self.dim)
-            dw = torch.empty_like(w)
-            a.weight, a.dx, a.dweight = w.data_ptr(), dx.data_ptr(), dw.data_ptr()
+            a.weight, a.dx = w.data_ptr(), dx.data_ptr()
+            if need_w:
+                dw = torch.empty_like(w)
+                a.dweight = dw.data_ptr()
             if h is not None:
                 a.h, a.ldh = a.x, a.ldx = h.data_ptr(), h.stride(0)
         a.stats = stats.data_ptr()
         if codes is not None:
             a.codes, a.ld_codes = codes.data_ptr(), self.code_bytes
         if rows:
-            n = max(_lib.lib().cueq_b200_norm_parts(C.byref(a)), 0)
-            parts = stats.new_empty(n)
-            a.parts, a.parts_values = parts.data_ptr(), n
+            a.parts_values = -1
+            if ds is not None or dw is not None:
+                n = max(_lib.lib().cueq_b200_norm_parts(C.byref(a)), 0)
+                parts = stats.new_empty(n)
+                a.parts, a.parts_values = parts.data_ptr(), n
             self.launch("backward", a, like.device)
         else:
             ds, dw = (None if t is None else t.zero_() for t in (ds, dw))
@@ -220,8 +226,9 @@ def _gradients(ctx, *grads):
     if go is None and gn is None:
         return (None,) * 6
     y, g, h, codes, stats, s, w = ctx.saved_tensors
-    grads = block.backward(go, gn, y, g, h, codes, stats, s, w)
-    return (None, *(t if need else None for t, need in zip(grads, ctx.needs_input_grad[1:])))
+    need = ctx.needs_input_grad[1:]
+    grads = block.backward(go, gn, y, g, h, codes, stats, s, w, need[3], need[4])
+    return (None, *(t if n else None for t, n in zip(grads, need)))
 
 
 _gradients_once = torch.autograd.function.once_differentiable(_gradients)

@@ -616,7 +616,8 @@ int cueq_b200_selftest_bounded_wait(void* status, void* waited_cycles, void* str
  * type, and with `codes` (16- and 32-bit data) what the backward pass reads of y (alone: x), g and out in 8 bits: rows of ld_codes
  * bytes, at least cueq_b200_norm_code_bytes().  The backward pass takes the same stats and either codes or the operands
  * themselves (`h`: x or out; BOTH on 16-bit data: `x` and no `h`, as out has been rounded), the cotangents go (of out; nullable with BOTH) and gn (of norm), and writes dx (BRANCH: not
- * written, it is go), dy, dg, dscale, dweight.  `parts`: cueq_b200_norm_parts() values of the arithmetic's type. */
+ * written, it is go), dy, dg, dscale, dweight (these two nullable).  `parts`:
+ * cueq_b200_norm_parts() values of the arithmetic's type; parts_values -1 and no parts where neither dscale nor dweight is wanted. */
 #define CUEQ_NORM_MAX_BLOCKS 64
 #define CUEQ_NORM_BRANCH 1
 #define CUEQ_NORM_ALONE 2
