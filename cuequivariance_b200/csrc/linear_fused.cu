@@ -41,7 +41,7 @@ constexpr int kMaxPaths = CUEQ_LINEAR_MAX_PATHS, kMaxClasses = CUEQ_LINEAR_MAX_C
 constexpr int kBlk = 128 * 128;              // one operand block: 128 rows x 32 float32, 16 KiB
 constexpr int kMaxRunGw = 128;               // K blocks per run of linear_gw
 
-struct LPath { int x_off, o_off, w_off, K, N, d, w_sn, w_sk; float c; int code_off; };
+struct LPath { int x_off, o_off, w_off, K, N, d, w_sn, w_sk; float c; int code_off, items; };   // items: tiles or K blocks over all classes
 
 struct LParams {
   const float* x;       // linear_map: input rows; linear_gw: x rows (M side)
@@ -504,11 +504,10 @@ __device__ __forceinline__ void gw_steps(const float* raw, unsigned char* hi, in
 // the K block in which the cost of all blocks before reaches `cost`
 template <bool CODES>
 __device__ __forceinline__ int gw_item(const LParams& p, int64_t cost) {
+  if (!CODES) return (int)cost;              // every block costs 1; walking the paths and classes for that cost 241 us for 168 (64 classes, 8 irreps, 4,096 rows)
   int start = 0;
   for (int q = 0; q < p.num_paths; ++q) {
-    const int n = rows_per_block(p.path[q].d), w = gw_cost<CODES>(p.path[q].d);
-    int items = 0;
-    for (int c = 0; c < p.num_classes; ++c) items += (p.bounds[c + 1] - p.bounds[c] + n - 1) / n;
+    const int items = p.path[q].items, w = gw_cost<CODES>(p.path[q].d);
     if (cost < (int64_t)items * w) return start + (int)(cost / w);
     cost -= (int64_t)items * w;
     start += items;
@@ -711,7 +710,10 @@ int make_params(const cueq_linear_args* a, PerItem per_item, bool gw, LParams* p
     } else {
       q.K = s.u; q.N = s.v; q.x_off = s.x_off; q.o_off = s.out_off; q.w_sn = 1; q.w_sk = s.v;
     }
-    for (int c = 0; c < a->num_classes; ++c) total += (a->bounds[c + 1] - a->bounds[c] + per_item(s.d) - 1) / per_item(s.d);
+    int64_t items = 0;
+    for (int c = 0; c < a->num_classes; ++c) items += (a->bounds[c + 1] - a->bounds[c] + per_item(s.d) - 1) / per_item(s.d);
+    q.items = (int)items;
+    total += items;
   }
   if (total > 2147483647LL) return cueq::fail("linear: too many rows");
   p->total = (int)total;
@@ -732,8 +734,7 @@ int gw_blocks(const LParams& p) {
 template <bool CODES>
 int64_t gw_total_cost(const LParams& p) {
   int64_t cost = 0;
-  for (int k = 0; k < p.num_paths; ++k)
-    for (int c = 0; c < p.num_classes; ++c) cost += (int64_t)gw_cost<CODES>(p.path[k].d) * ((p.bounds[c + 1] - p.bounds[c] + rows_per_block(p.path[k].d) - 1) / rows_per_block(p.path[k].d));
+  for (int k = 0; k < p.num_paths; ++k) cost += (int64_t)gw_cost<CODES>(p.path[k].d) * p.path[k].items;
   return cost;
 }
 // the larger of the two ways to divide the blocks, so that one size of `parts` serves both
