@@ -123,6 +123,9 @@ int make_plan(const cueq_norm_args* a, bool backward, bool dense, Params* p, int
   }
   if (p->dim_total * size % 16 || (gated(a) && p->channels * size % 16)) even = false;
   p->num_slices = ns; p->nb = a->num_blocks;
+  // sizes from here on stay below a few MB: every pass has a row of a slice's values in shared memory
+  for (int k = 0; k < ns; ++k)
+    if ((int64_t)p->slice[k].values * size > kSmemPerSm) return dense && p->slice[k].count > 1 ? kTooLongForUnits : kTooLong;
   set_routes(a, backward, p, dense && ns == 1, even);
   int unit = 1;                                          // rows after which dense rows are on a 16-byte boundary again
   if (dense && ns == 1) while (unit < 8 && (unit * p->dim_total * size % 16 || (gated(a) && unit * p->channels * size % 16))) unit *= 2;
@@ -195,7 +198,7 @@ int fill(const cueq_norm_args* a, bool backward, Params* p, int* grid, int* smem
     code_layout(a, p);
     rc = make_plan(a, backward, dense, p, grid, smem);
   }
-  if (rc) return cueq::fail("norm: an irrep block does not fit into shared memory (%d bytes of %d)", *smem, kSmemPerSm);
+  if (rc) return cueq::fail("norm: a row of an irrep block does not fit into shared memory (%d bytes)", kSmemPerSm);
   return 0;
 }
 
