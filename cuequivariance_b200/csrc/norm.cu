@@ -251,6 +251,13 @@ Kernel pick_kernel(int dtype, int mode, bool q8, bool mul_ir, bool backward) {
 int launch(const cueq_norm_args* a, bool backward, void* stream) {
   Params p;
   int grid = 0, smem = 0;
+  if (!backward && a && a->stats) {                      // a backward pass is to come: it has to fit as well, and only long blocks do not
+    if (int rc = check(a)) return rc;
+    int longest = 0;
+    for (int k = 0; k < a->num_blocks; ++k) { const int n = a->blocks[k].mul * a->blocks[k].dim; longest = n > longest ? n : longest; }
+    if (longest > kSliceValues)
+      if (int rc = fill(a, true, &p, &grid, &smem)) return rc;
+  }
   if (int rc = fill(a, backward, &p, &grid, &smem)) return rc;
   const bool branch = a->mode & kBranch, norm = a->mode & kNorm;
   const int64_t width = p.dim_total, channels = p.channels;

@@ -258,7 +258,9 @@ class IrrepsNorm(torch.nn.Module):
 
     ``weight``: ``[irreps.num_irreps]``, channels in the order of the blocks; the module's own parameter when ``internal_weights``
     (ones at first).  float64 features go with float64 weights; others with weights of any other type.  Arithmetic, statistics and
-    sums are in 32 bits (64 for float64); results are rounded once.  Rows may lie further apart than their width.
+    sums are in 32 bits (64 for float64); results are rounded once.  Rows may lie further apart than their width.  A row of an irrep block
+    has to fit into the shared memory of an SM: up to 14,000 channels of scalars or 3,600 of l = 3 in float32 with a gradient to come, half
+    of that in float64; longer blocks raise in the forward pass.
 
     ``saved_activations="int8"`` (not for float64) keeps x in 8 bits for the backward pass, per row and irrep block with a step of a power of two (off by at most
     1/127 of the block's largest magnitude); the forward result does not change.  First derivatives only, and none in forward mode."""
@@ -289,7 +291,8 @@ class GatedResidual(torch.nn.Module):
     required unless ``gate`` is None (``"sigmoid"``, ``"silu"``); ``scale``, ``weight``: ``[irreps.num_irreps]``, the module's own parameters when
     ``internal_weights`` (``initial_scale`` and ones at first).  ``norm`` is ``IrrepsNorm`` without weights - ``scale`` is its weight.
 
-    Types, rows, rounding and ``saved_activations`` as in ``IrrepsNorm``; in 8 bits are kept ``update``, ``gates`` and with ``norm_output`` the result.
+    Blocks of up to 9,600 channels of scalars or 3,200 of l = 3 in float32, 5,700 or 1,700 with ``norm_output``, half of that in float64.  Types,
+    rows, rounding and ``saved_activations`` as in ``IrrepsNorm``; in 8 bits are kept ``update``, ``gates`` and with ``norm_output`` the result.
     One pass each way: with ``norm_output`` the sum is neither read again for its norm nor its two gradients added by another pass."""
 
     def __init__(self, irreps, *, layout=None, gate: Optional[str] = "sigmoid", norm_output: bool = False, eps: float = 1e-5,

@@ -26,3 +26,19 @@ def test_no_length_wraps_around(mul, count, mode, dtype):
     a = _args(mode, ((mul, 1),) * count, dtype)
     assert _lib.lib().cueq_b200_norm_parts(C.byref(a)) == -1
     assert "shared memory" in _lib.lib().cueq_b200_last_error().decode()
+
+
+@pytest.mark.parametrize("mode,blocks,dtype", [
+    (_lib.NORM_BOTH, ((1024, 7),), 1), (_lib.NORM_ALONE, ((20000, 1),), 0), (_lib.NORM_BRANCH, ((12000, 1),), 0), (_lib.NORM_BOTH, ((8, 3), (4000, 5)), 2),
+])
+def test_a_forward_pass_whose_gradient_would_not_fit(mode, blocks, dtype):
+    """Refused where statistics are kept for a backward pass, run where none are.  No rows: nothing is launched."""
+    L = _lib.lib()
+    width = sum(m * d for m, d in blocks)
+    a = _args(mode, blocks, dtype, x=16, ldx=width, y=16, ldy=width, scale=16, weight=16, out=16, norm=16)
+    a.rows = 0
+    assert L.cueq_b200_norm_parts(C.byref(a)) == -1
+    assert L.cueq_b200_norm_forward(C.byref(a), None) == 0
+    a.stats = 16
+    assert L.cueq_b200_norm_forward(C.byref(a), None) != 0
+    assert "shared memory" in L.cueq_b200_last_error().decode()
