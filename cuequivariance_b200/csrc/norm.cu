@@ -207,11 +207,13 @@ struct SumParams {
   const void* parts;
   void* out[2];
   int warps, channels, dtype;
+  const int* status;
 };
 constexpr int kSumRows = 128, kSumChannels = 8;   // eight channels, a sector of a warp's sums; 1,800 warps in 14 steps (32 x 32 threads: 50 steps, 8 us)
 template <class M>
 __global__ void __launch_bounds__(kSumChannels * kSumRows) sum_kernel(const __grid_constant__ SumParams p) {
   __shared__ M partial[kSumRows][kSumChannels + 1];
+  if (!cueq_tc::status_clean(p.status)) return;           // a warp that gave up has left no sums
   const int ch = blockIdx.x * kSumChannels + threadIdx.x;
   const int which = blockIdx.y;
   M v = M(0);
@@ -303,7 +305,7 @@ int launch(const cueq_norm_args* a, bool backward, void* stream) {
     CUEQ_CUDA_OK(cudaGetLastError());
   }
   if (!backward) return 0;
-  SumParams s{a->parts, {branch ? a->dscale : nullptr, norm ? a->dweight : nullptr}, a->rows ? grid : 0, p.channels, a->param_dtype};
+  SumParams s{a->parts, {branch ? a->dscale : nullptr, norm ? a->dweight : nullptr}, a->rows ? grid : 0, p.channels, a->param_dtype, p.status};
   if (!s.out[0] && !s.out[1]) return 0;
   const dim3 g((p.channels + kSumChannels - 1) / kSumChannels, 2), t(kSumChannels, kSumRows);
   if (a->dtype == CUEQ_F64) sum_kernel<double><<<g, t, 0, st>>>(s);

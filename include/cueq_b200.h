@@ -645,7 +645,8 @@ typedef struct {
   void* stats;
   void* parts;
   int64_t parts_values;
-  void* status;                  /* nullable device int32: 2 if a bounded wait ran out              */
+  void* status;                  /* nullable device int32: 2 if a bounded wait ran out; dscale, dweight
+                                    are not written then                                              */
 } cueq_norm_args;
 int64_t cueq_b200_norm_code_bytes(const cueq_norm_args* args);
 int64_t cueq_b200_norm_stats(const cueq_norm_args* args);
