@@ -302,8 +302,9 @@ class Linear(torch.nn.Module):
     flattened over ``u``.  There is no ``naive`` method and no fallback.
 
     ``saved_activations="int8"`` keeps x in 8 bits for the weight gradient, per row and irrep block with a step of a power of two (off
-    by at most 1/127 of the block's largest magnitude); the output and the input gradient do not change, the weight gradient is that of the kept
-    values.  It is for what the fused launches take (first sentence above, any number of rows); other shapes, types and unsorted
+    by at most 1/127 of the block's largest magnitude); the output and the input gradient do not change (but for rounding below 256 rows, which
+    take the tensor-core launches here and the generic kernel there), the weight gradient is that of the kept values: of a rotated input
+    it is another one, within the same bound.  It is for what the fused launches take (first sentence above, any number of rows); other shapes, types and unsorted
     classes raise."""
 
     def __init__(

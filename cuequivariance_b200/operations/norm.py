@@ -7,7 +7,12 @@ No counterpart in the reference.  Features are rows of irrep blocks (mul channel
 * ``GatedResidual``: ``h = x + s act(g) y r(y)`` for the block's output ``y``, one gate per row and channel, one scale per channel;
   with ``norm_output`` also ``n = w h r(h)``, the norm in front of the next block, in the same pass.
 
-A block's components share their factors, so both are equivariant.  The kernels are ``csrc/norm_kernels.cuh``.
+A block's components share their factors, so both are equivariant, and so are their gradients with activations kept in full.  With
+``saved_activations="int8"`` the forward results still are; the gradients are not: the step of a block follows its largest component, which a
+rotation changes, so a gradient is off by up to 1/127 in a direction that depends on the frame.  Forces from such gradients are neither covariant nor
+exactly a derivative of the energy.
+
+The kernels are ``csrc/norm_kernels.cuh``.
 """
 from __future__ import annotations
 
@@ -258,12 +263,14 @@ class IrrepsNorm(torch.nn.Module):
 
     ``weight``: ``[irreps.num_irreps]``, channels in the order of the blocks; the module's own parameter when ``internal_weights``
     (ones at first).  float64 features go with float64 weights; others with weights of any other type.  Arithmetic, statistics and
-    sums are in 32 bits (64 for float64); results are rounded once.  Rows may lie further apart than their width.  A row of an irrep block
+    sums are in 32 bits (64 for float64); results are rounded once; a block whose sum of squares leaves that range (values from 1e19 on
+    in float32 and bfloat16) counts as infinitely long and becomes zeros.  Rows may lie further apart than their width.  A row of an irrep block
     has to fit into the shared memory of an SM: up to 14,000 channels of scalars or 3,600 of l = 3 in float32 with a gradient to come, half
     of that in float64; longer blocks raise in the forward pass.
 
     ``saved_activations="int8"`` (not for float64) keeps x in 8 bits for the backward pass, per row and irrep block with a step of a power of two (off by at most
-    1/127 of the block's largest magnitude); the forward result does not change.  First derivatives only, and none in forward mode."""
+    1/127 of the block's largest magnitude); the forward result does not change; the gradients are then not equivariant: not for forces.
+    First derivatives only, and none in forward mode."""
 
     def __init__(self, irreps, *, layout=None, eps: float = 1e-5, internal_weights: bool = True, saved_activations: str = "full",
                  device: Optional[torch.device] = None, dtype: Optional[torch.dtype] = None):
@@ -289,7 +296,7 @@ class GatedResidual(torch.nn.Module):
 
     ``x``, ``update``: ``[batch, irreps.dim]``; ``gates``: ``[batch, irreps.num_irreps]``, one per channel in the order of the blocks,
     required unless ``gate`` is None (``"sigmoid"``, ``"silu"``); ``scale``, ``weight``: ``[irreps.num_irreps]``, the module's own parameters when
-    ``internal_weights`` (``initial_scale`` and ones at first).  ``norm`` is ``IrrepsNorm`` without weights - ``scale`` is its weight.
+    ``internal_weights`` (``initial_scale`` and ones at first).  Gates below -87 are closed: both activations are 0 there.  ``norm`` is ``IrrepsNorm`` without weights - ``scale`` is its weight.
 
     Blocks of up to 9,600 channels of scalars or 3,200 of l = 3 in float32, 5,700 or 1,700 with ``norm_output``, half of that in float64.  Types,
     rows, rounding and ``saved_activations`` as in ``IrrepsNorm``; in 8 bits are kept ``update``, ``gates`` and with ``norm_output`` the result.
