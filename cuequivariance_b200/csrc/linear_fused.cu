@@ -12,7 +12,8 @@
 // What bounds them: the rows are read once and written once, 2 * 268 MB each for 32,768 nodes of 128x(0e+1o+2e+3o);
 // 82 us at 6.5 TB/s against 46 us of three-pass TF32.  The layer used to be one GEMM launch per irrep and component
 // (48 of them, the row reductions on 32 thread blocks), with layout transpositions around them and the weights split by
-// elementwise kernels: 3.25 ms for forward and both gradients.  Now 0.62 ms: linear_map 195 us (2.75 TB/s), linear_gw 212 us, with x in codes 153 us (and 58 us to write them).
+// elementwise kernels: 3.25 ms for forward and both gradients.  Now 0.63 ms: linear_map 200 us (2.7 TB/s), linear_gw 231 us, with x in codes 153 us (and 58 us to write them); with
+// the nodes in 64 classes linear_map 270-280 us, linear_gw 254 and 195 us.
 // What is left is the latency between load, split and MMA: tensor pipe 23 % and HBM 45 % busy.
 //
 // The components of an irrep share its weight block, so rows (z, i) are folded into the M axis of the MMA (linear_map)

@@ -251,7 +251,7 @@ class _FusedLinear(torch.autograd.Function):
         gout = _aligned(gout)
         gw = gx = None
         if ctx.needs_input_grad[3]:
-            gx = (torch.empty if plan["full_in"] and ctx.all_rows else torch.zeros)((ctx.rows, plan["in_size"]), dtype=torch.float32, device=gout.device)
+            gx = (gout.new_empty if plan["full_in"] and ctx.all_rows else gout.new_zeros)((ctx.rows, plan["in_size"]))
             _FusedLinear._launch(plan, "map", bounds, gout, weight, gx, transposed=1)
         if ctx.needs_input_grad[2]:
             # the weights are the blocks of the paths, all of them written; without any row nothing is
