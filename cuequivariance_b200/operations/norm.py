@@ -299,7 +299,8 @@ class GatedResidual(torch.nn.Module):
     ``internal_weights`` (``initial_scale`` and ones at first).  Gates below -87 are closed: both activations are 0 there.  ``norm`` is ``IrrepsNorm`` without weights - ``scale`` is its weight.
 
     Blocks of up to 9,600 channels of scalars or 3,200 of l = 3 in float32, 5,700 or 1,700 with ``norm_output``, half of that in float64.  Types,
-    rows, rounding and ``saved_activations`` as in ``IrrepsNorm``; in 8 bits are kept ``update``, ``gates`` and with ``norm_output`` the result.
+    rows, rounding and ``saved_activations`` as in ``IrrepsNorm``.  Kept for the gradient are ``update``, ``gates`` and with ``norm_output`` the result, but in
+    16 bits ``x`` in its place (the result has been rounded); in 8 bits ``update``, ``gates`` and the result before it was rounded.
     One pass each way: with ``norm_output`` the sum is neither read again for its norm nor its two gradients added by another pass."""
 
     def __init__(self, irreps, *, layout=None, gate: Optional[str] = "sigmoid", norm_output: bool = False, eps: float = 1e-5,
